@@ -64,6 +64,9 @@ SIGNATURES = {
     "gdn2_layer_step_workspace_bytes": (_sz, [_i64] * 7 + [_int]),
     "gdn2_layer_step": (_int, [_vp, _int, _vp]),
     "gdn2_layer_back": (_int, [_vp] * 4 + [_i64] * 5 + [_f32, _int, _vp]),
+    "gdn2_recurrence_marks": (_sz, [_i64, _i64, ctypes.POINTER(_i64), _i64]),
+    "gdn2_recurrence_forward": (_int, [_vp, _int, _vp]),
+    "gdn2_recurrence_backward": (_int, [_vp, _int, _vp]),
 }
 
 
@@ -99,6 +102,16 @@ class OProjReduceArgs(ctypes.Structure):
 
     _fields_ = ([(n, _vp) for n in ("x", "weight", "out", "peer_slots", "peer_flags", "epochs")]
                 + [(n, _i64) for n in ("rows", "K", "hidden")] + [("rank", _int), ("world", _int), ("wait_cycles", _i64)])
+
+
+class RecurrenceArgs(ctypes.Structure):
+    """``gdn2_recurrence_args`` of include/gdn2_b200.h."""
+
+    _fields_ = ([(n, _vp) for n in ("v", "g", "w", "state", "o", "final_state", "marks", "dout", "dfinal_state", "dv", "dg", "dw",
+                                    "dstate")]
+                + [("cu_seqlens", ctypes.POINTER(_i64))]
+                + [(n, _i64) for n in ("sequences", "B", "S", "D", "v_batch_stride", "v_token_stride", "g_batch_stride",
+                                       "g_token_stride", "w_batch_stride", "w_token_stride", "do_batch_stride", "do_token_stride")])
 
 
 _lock = threading.Lock()
@@ -209,6 +222,18 @@ def _seq_view(t: torch.Tensor):
             return t, (t.stride(0) // (H * D) if B > 1 else S)
     t = t.contiguous()
     return t, S
+
+
+def _rows_view(t: torch.Tensor):
+    """``(tensor, batch stride, token stride)`` in elements of ``[B, S, D]`` rows whose channels lie side by side; copied if
+    they do not. The stride of a dimension of one entry is never used and given as 0."""
+    if t.shape[2] > 1 and t.stride(2) != 1:
+        t = t.contiguous()
+    return t, (t.stride(0) if t.shape[0] > 1 else 0), (t.stride(1) if t.shape[1] > 1 else 0)
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
 
 
 class NativeKernels:
@@ -522,6 +547,71 @@ class NativeKernels:
             _check(self.lib, rc, "gdn2_chunk_output")
         self.launches += 3 if p != PATH_SIMT else 2
         return out
+
+    # -- diagonal recurrence -----------------------------------------------------------------
+    @staticmethod
+    def _recurrence_args(v, g, w, offsets):
+        """The argument structure with inputs and sizes filled in, and what has to stay alive until the call."""
+        a = RecurrenceArgs()
+        keep = []
+        for name, t in (("v", v), ("g", g), ("w", w)):
+            if t is not None:
+                t, bs, ts = _rows_view(t)
+                keep.append(t)
+                setattr(a, name, t.data_ptr())
+                setattr(a, f"{name}_batch_stride", bs)
+                setattr(a, f"{name}_token_stride", ts)
+        a.B, a.S, a.D = v.shape
+        a.sequences = a.B
+        if offsets is not None:
+            a.sequences = len(offsets) - 1
+            cu = (_i64 * len(offsets))(*offsets)
+            keep.append(cu)
+            a.cu_seqlens = cu
+        return a, keep
+
+    def _recurrence_launches(self, a) -> int:
+        return -(-a.sequences // 128) if a.cu_seqlens else 1
+
+    def recurrence(self, v, g, w, state, offsets, want_final=True, want_marks=False, in_place=False):
+        """``gdn2_recurrence_forward`` on ``[B, S, D]`` rows (``g`` float32): ``(o, final_state | None, marks | None)``. ``state``:
+        float32 ``[sequences, D]`` or ``None``; with ``in_place`` the final state is written into it."""
+        _require_cuda(v, g, w, state)
+        a, keep = self._recurrence_args(v, g, w, offsets)
+        dev = v.device
+        if state is not None and not state.is_contiguous():
+            state = state.contiguous()
+        o = torch.empty(v.shape, dtype=v.dtype, device=dev)
+        final = state if in_place else torch.empty(a.sequences, a.D, dtype=torch.float32, device=dev) if want_final else None
+        marks = None
+        if want_marks:
+            rows = self.lib.gdn2_recurrence_marks(a.B, a.S, a.cu_seqlens, a.sequences)
+            marks = torch.empty(rows, a.D, dtype=torch.float32, device=dev)
+        a.state, a.o, a.final_state, a.marks = _ptr(state), o.data_ptr(), _ptr(final), _ptr(marks)
+        with _on_device(dev):
+            rc = self.lib.gdn2_recurrence_forward(ctypes.byref(a), dtype_code(v.dtype), self._stream(v))
+        _check(self.lib, rc, "gdn2_recurrence_forward")
+        self.launches += self._recurrence_launches(a)
+        return o, final, marks
+
+    def recurrence_backward(self, v, g, w, marks, do, dfinal, offsets, want_dstate):
+        """``gdn2_recurrence_backward``: ``(dv, dg, dw | None, dstate | None)``."""
+        _require_cuda(v, g, w, marks, do, dfinal)
+        a, keep = self._recurrence_args(v, g, w, offsets)
+        dev = v.device
+        do, a.do_batch_stride, a.do_token_stride = _rows_view(do)
+        dfinal = None if dfinal is None else dfinal.contiguous()
+        dv = torch.empty(v.shape, dtype=v.dtype, device=dev)
+        dg = torch.empty(v.shape, dtype=torch.float32, device=dev)
+        dw = None if w is None else torch.empty_like(dv)
+        dstate = torch.empty(a.sequences, a.D, dtype=torch.float32, device=dev) if want_dstate else None
+        a.marks, a.dout, a.dfinal_state = marks.data_ptr(), do.data_ptr(), _ptr(dfinal)
+        a.dv, a.dg, a.dw, a.dstate = dv.data_ptr(), dg.data_ptr(), _ptr(dw), _ptr(dstate)
+        with _on_device(dev):
+            rc = self.lib.gdn2_recurrence_backward(ctypes.byref(a), dtype_code(v.dtype), self._stream(v))
+        _check(self.lib, rc, "gdn2_recurrence_backward")
+        self.launches += self._recurrence_launches(a)
+        return dv, dg, dw, dstate
 
     # -- diagnostics -------------------------------------------------------------------------
     def check_device_status(self, device=None):

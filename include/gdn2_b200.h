@@ -418,6 +418,47 @@ typedef struct gdn2_oproj_reduce_args {
 size_t gdn2_oproj_reduce_buffer_bytes(int64_t world, int64_t hidden, size_t* flags_offset);
 int gdn2_oproj_reduce(const gdn2_oproj_reduce_args* args, int dtype, void* stream);
 
+/*
+ * Diagonal gated recurrence: per sequence and channel h_t = exp(g_t) h_{t-1} + w_t v_t, o_t = h_t, evaluated in fp32.
+ *   v, w [B, S, D]  g [B, S, D] fp32 natural-log decay, <= 0 (-inf: the state is forgotten)  o [B, S, D]
+ *   state, final_state [sequences, D] fp32
+ * w == NULL: no write gate (w_t = 1). state == NULL: zeros. The channels of a token are contiguous; tokens and batch entries
+ * are `*_token_stride` / `*_batch_stride` ELEMENTS apart in v, w, g and dout, so columns of a wider projection are passed as
+ * they are. o, dv, dw, dg are contiguous. Without cu_seqlens a sequence is a batch entry (sequences = B). With cu_seqlens, a
+ * HOST array of sequences + 1 token offsets rising from 0 to S, the sequences are packed along the token axis and B is 1.
+ * `marks`: NULL, or [gdn2_recurrence_marks(...), D] fp32 that the forward call fills with the state that enters every 64th
+ * token of a sequence, for the backward call. final_state may be state: decoding in place, S tokens at a time.
+ * gdn2_recurrence_backward: dv, dw (NULL without w), dg [B, S, D] and dstate (may be NULL) from dout and dfinal_state (NULL:
+ * zeros); v, g, w, state strides and marks as in the forward call.
+ * Any D >= 1, B >= 1, S >= 1, any alignment of elements; 16-byte aligned rows of a multiple of 16 bytes take the fast kernels.
+ * No counterpart in the reference, whose only token mixer is the delta rule's (its decay convention is this one's).
+ */
+typedef struct gdn2_recurrence_args {
+  const void* v;
+  const float* g;
+  const void* w;
+  const float* state;
+  void* o;
+  float* final_state;
+  float* marks;
+  const void* dout;
+  const float* dfinal_state;
+  void* dv;
+  float* dg;
+  void* dw;
+  float* dstate;
+  const int64_t* cu_seqlens;
+  int64_t sequences;
+  int64_t B, S, D;
+  int64_t v_batch_stride, v_token_stride, g_batch_stride, g_token_stride, w_batch_stride, w_token_stride;
+  int64_t do_batch_stride, do_token_stride;
+} gdn2_recurrence_args;
+
+/* Rows of `marks`: 64-token pieces, counted per sequence. */
+size_t gdn2_recurrence_marks(int64_t B, int64_t S, const int64_t* cu_seqlens, int64_t sequences);
+int gdn2_recurrence_forward(const gdn2_recurrence_args* args, int dtype, void* stream);
+int gdn2_recurrence_backward(const gdn2_recurrence_args* args, int dtype, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
