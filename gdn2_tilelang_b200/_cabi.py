@@ -67,7 +67,11 @@ SIGNATURES = {
     "gdn2_recurrence_marks": (_sz, [_i64, _i64, ctypes.POINTER(_i64), _i64]),
     "gdn2_recurrence_forward": (_int, [_vp, _int, _vp]),
     "gdn2_recurrence_backward": (_int, [_vp, _int, _vp]),
+    "gdn2_ffn_forward": (_int, [_vp, _int, _vp]),
+    "gdn2_ffn_backward": (_int, [_vp, _int, _vp]),
+    "gdn2_align_rows": (_int, [_vp, _i64, _vp]),
 }
+ACTIVATIONS = {"silu": 0, "gelu_tanh": 1}
 
 
 class LayerFrontArgs(ctypes.Structure):
@@ -112,6 +116,22 @@ class RecurrenceArgs(ctypes.Structure):
                 + [("cu_seqlens", ctypes.POINTER(_i64))]
                 + [(n, _i64) for n in ("sequences", "B", "S", "D", "v_batch_stride", "v_token_stride", "g_batch_stride",
                                        "g_token_stride", "w_batch_stride", "w_token_stride", "do_batch_stride", "do_token_stride")])
+
+
+class FfnArgs(ctypes.Structure):
+    """``gdn2_ffn_args`` of include/gdn2_b200.h."""
+
+    _fields_ = ([(n, _vp) for n in ("x", "w_gate", "w_up", "w_down", "h", "a", "u", "y", "dy", "da", "du", "dx", "dw_gate", "dw_up",
+                                    "dw_down")]
+                + [(n, _i64) for n in ("tokens", "hidden", "inner", "out", "x_stride", "w_gate_stride", "w_up_stride",
+                                       "w_down_stride", "inner_stride", "y_stride", "dy_stride", "dx_stride")]
+                + [("activation", _int)])
+
+
+class RowCopy(ctypes.Structure):
+    """``gdn2_row_copy`` of include/gdn2_b200.h."""
+
+    _fields_ = [("src", _vp), ("dst", _vp)] + [(n, _i64) for n in ("rows", "cols", "src_stride", "dst_stride")]
 
 
 _lock = threading.Lock()
@@ -230,6 +250,11 @@ def _rows_view(t: torch.Tensor):
     if t.shape[2] > 1 and t.stride(2) != 1:
         t = t.contiguous()
     return t, (t.stride(0) if t.shape[0] > 1 else 0), (t.stride(1) if t.shape[1] > 1 else 0)
+
+
+def _pitch(t: torch.Tensor) -> int:
+    """Elements from one row of an aligned matrix to the next (of a single row: the row padded to 16 bytes)."""
+    return t.stride(0) if t.shape[0] > 1 else -(-t.shape[1] // 8) * 8
 
 
 def _ptr(t):
@@ -612,6 +637,70 @@ class NativeKernels:
         _check(self.lib, rc, "gdn2_recurrence_backward")
         self.launches += self._recurrence_launches(a)
         return dv, dg, dw, dstate
+
+    # -- gated feed-forward ------------------------------------------------------------------
+    def aligned_rows(self, *matrices):
+        """``[rows, cols]`` matrices of 16-bit elements as the tensor-core kernels read them: rows that start on 16 bytes and whose
+        elements lie side by side. Those that do not are copied, all in one launch."""
+        out, copies = list(matrices), []
+        for i, t in enumerate(matrices):
+            if t.shape[1] > 1 and t.stride(1) != 1:
+                t = out[i] = t.contiguous()
+            one = t.shape[0] == 1
+            if t.data_ptr() % 16 or (not one and (t.stride(0) % 8 or t.stride(0) < t.shape[1])):
+                pitch = -(-t.shape[1] // 8) * 8
+                out[i] = torch.empty(t.shape[0], pitch, dtype=t.dtype, device=t.device)[:, :t.shape[1]]
+                copies.append(RowCopy(t.data_ptr(), out[i].data_ptr(), *t.shape, 0 if one else t.stride(0), pitch))
+        if copies:
+            with _on_device(out[0].device):
+                rc = self.lib.gdn2_align_rows((RowCopy * len(copies))(*copies), len(copies), self._stream(out[0]))
+            _check(self.lib, rc, "gdn2_align_rows")
+            self.launches += 1
+        return out
+
+    @staticmethod
+    def _ffn_args(x, w_gate, w_up, w_down, activation):
+        a = FfnArgs()
+        a.x, a.w_gate, a.w_up, a.w_down = (t.data_ptr() for t in (x, w_gate, w_up, w_down))
+        a.tokens, a.hidden = x.shape
+        a.out, a.inner = w_down.shape
+        a.x_stride, a.w_gate_stride, a.w_up_stride, a.w_down_stride = (_pitch(t) for t in (x, w_gate, w_up, w_down))
+        a.inner_stride = -(-a.inner // 8) * 8
+        a.activation = ACTIVATIONS[activation]
+        return a
+
+    def ffn_forward(self, x, w_gate, w_up, w_down, activation: str, keep: bool):
+        """``gdn2_ffn_forward`` on rows as ``aligned_rows`` leaves them: ``(y [tokens, out], h, a, u)``; the kept buffers have rows of
+        ``inner`` elements padded to a multiple of 8 (``a``, ``u``: ``None`` without ``keep``)."""
+        a = self._ffn_args(x, w_gate, w_up, w_down, activation)
+        rows = lambda: torch.empty(a.tokens, a.inner_stride, dtype=x.dtype, device=x.device)     # noqa: E731
+        y = torch.empty(a.tokens, a.out, dtype=x.dtype, device=x.device)
+        h, gate, up = rows(), (rows() if keep else None), (rows() if keep else None)
+        a.h, a.a, a.u, a.y, a.y_stride = h.data_ptr(), _ptr(gate), _ptr(up), y.data_ptr(), a.out
+        with _on_device(x.device):
+            rc = self.lib.gdn2_ffn_forward(ctypes.byref(a), dtype_code(x.dtype), self._stream(x))
+        _check(self.lib, rc, "gdn2_ffn_forward")
+        self.launches += 2
+        return y, h, gate, up
+
+    def ffn_backward(self, x, w_gate, w_up, w_down, h, gate, up, dy, activation: str, want_dx: bool, want_dgate_up: bool,
+                     want_dw_down: bool):
+        """``gdn2_ffn_backward``: ``(dx, dw_gate, dw_up, dw_down)``, ``None`` where not wanted."""
+        a = self._ffn_args(x, w_gate, w_up, w_down, activation)
+        new = lambda *shape: torch.empty(*shape, dtype=x.dtype, device=x.device)                 # noqa: E731
+        first = want_dx or want_dgate_up
+        da, du = (new(a.tokens, a.inner_stride), new(a.tokens, a.inner_stride)) if first else (None, None)
+        dx = new(a.tokens, a.hidden) if want_dx else None
+        dwg, dwu = (new(a.inner, a.hidden), new(a.inner, a.hidden)) if want_dgate_up else (None, None)
+        dwd = new(a.out, a.inner) if want_dw_down else None
+        a.h, a.a, a.u, a.dy, a.dy_stride = h.data_ptr(), gate.data_ptr(), up.data_ptr(), dy.data_ptr(), _pitch(dy)
+        a.da, a.du, a.dx, a.dx_stride = _ptr(da), _ptr(du), _ptr(dx), a.hidden
+        a.dw_gate, a.dw_up, a.dw_down = _ptr(dwg), _ptr(dwu), _ptr(dwd)
+        with _on_device(x.device):
+            rc = self.lib.gdn2_ffn_backward(ctypes.byref(a), dtype_code(x.dtype), self._stream(x))
+        _check(self.lib, rc, "gdn2_ffn_backward")
+        self.launches += int(first) + int(want_dx) + int(want_dgate_up) + int(want_dw_down)
+        return dx, dwg, dwu, dwd
 
     # -- diagnostics -------------------------------------------------------------------------
     def check_device_status(self, device=None):

@@ -1,0 +1,929 @@
+// The gated feed-forward block y = (act(x Wg^T) * (x Wu^T)) Wd^T and its gradient, 16-bit operands, fp32 accumulation.
+//
+//   forward   a = x Wg^T, u = x Wu^T, h = act(a) u     one kernel: both projections, the activation and the product
+//             y = h Wd^T
+//   backward  dh = dy Wd, da = dh u act'(a), du = dh act(a)      one kernel
+//             dx = da Wg + du Wu                                 one kernel (the two products are one long reduction)
+//             dWg = da^T x, dWu = du^T x;  dWd = dy^T h          a kernel each
+//
+// Every product is the same pipeline with another way in and another way out (product_kernel): a pair of blocks on two SMs
+// (cta_group::2) holds a 256 x 256 tile of the result in tensor memory, 128 rows each; TMA brings 64 reduction steps of both
+// operands a stage, each block its own 128 rows of A and its half of B's, six stages deep; one thread issues the products;
+// eight warps take the finished tile from tensor memory while the next one accumulates in the other half of it. The operands are read
+// as they lie in memory: with the reduction along rows (K-major) or down columns (MN-major), which the shared-memory
+// descriptors tell the tensor core, so nothing is transposed.
+//
+// In the forward product block 0 of a pair brings rows of Wg as its half of B and block 1 the same rows of Wu: columns c and 128 + c of
+// the tile are then the gate and the up projection of one inner channel, in the same lane of tensor memory, and the epilogue
+// needs nothing from another thread. h, and for a training step a and u, are rounded to 16 bits there: they are what the next
+// product reads, and a tensor core reads 16 bits. The sums before and after are fp32.
+//
+// Few tokens (skinny_kernel): the work is reading the weights once. They take the 128-row side of the product, the tokens
+// the narrow one, and the reduction of a tile is cut over the blocks of a cluster so that every SM reads; the blocks' partial
+// sums meet in distributed shared memory, added in the order of the blocks.
+#include <cuda.h>
+
+#include "common.cuh"
+#include "tc_utils.cuh"
+
+namespace gdn2 {
+
+namespace {
+
+constexpr int kTile = 256;                       // rows and columns of a pair's tile
+constexpr int kBlockRows = 128, kStep = 64;      // a block's rows of an operand, reduction steps of a stage
+constexpr int kOperandBytes = kBlockRows * kStep * 2;
+constexpr int kStageBytes = 2 * kOperandBytes;
+constexpr int kEpiWarps = 8, kThreads = (4 + kEpiWarps) * 32;
+constexpr int kChunk16 = 64;                     // columns of an epilogue chunk: 128 bytes
+constexpr int kChunkBytes = 32 * kChunk16 * 2;
+constexpr uint32_t kWaitCode = 1u << 28;
+
+enum Kind { kPlain = 0, kGated = 1, kGatedBackward = 2 };
+
+// Stages that fit beside a kind's staging buffers: one chunk a warp, two in and out for the backward epilogue.
+template <int K> __host__ __device__ constexpr int stages() { return K == kGatedBackward ? 5 : 6; }
+template <int K> __host__ __device__ constexpr int staging_bytes() { return kEpiWarps * kChunkBytes * (K == kGatedBackward ? 2 : 1); }
+template <int K> constexpr size_t smem_bytes() { return (size_t)stages<K>() * kStageBytes + staging_bytes<K>() + 1024; }
+
+struct __align__(64) Maps {
+  CUtensorMap a[2], b[2];       // kPlain: operands of the one or two runs of reduction steps; kGated: b = Wg, Wu
+  CUtensorMap out[3];           // kPlain: result (of the upper and of the lower tiles); kGated: h, a, u; kGatedBackward: da, du
+  CUtensorMap in[2];            // kGatedBackward: a, u
+};
+struct Problem {
+  int steps[2];                 // stages of the two runs (steps[1] = 0: one run)
+  int tiles_m, tiles_n;
+  int split_m;                  // > 0: tiles from this one on take a[1] and out[1], their rows counted from there (dWg, dWu)
+  int M, N;                     // rows and columns of the result (of one part)
+  int save, gelu;
+  void* plain_out[2];           // results whose rows do not start on 16 bytes are stored by threads
+  int64_t out_stride;
+};
+
+// ---------------------------------------------------------------- instructions
+
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ uint32_t in_block(uint32_t addr, uint32_t rank) {       // the same shared address in another block
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void tma_load_pair(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
+  asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%2, %3}], [%4];"
+               ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(bar) : "memory");
+}
+__device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
+  asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
+               ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(bar) : "memory");
+}
+__device__ __forceinline__ void tma_store(const CUtensorMap* map, int x, int y, uint32_t src) {
+  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%1, %2}], [%3];"
+               ::"l"(map), "r"(x), "r"(y), "r"(src) : "memory");
+}
+__device__ __forceinline__ void mma_pair(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+               "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+               ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+}
+// arrives on the barrier at this offset of both blocks once every product issued so far has completed
+__device__ __forceinline__ void commit_pair(uint64_t* bar) {
+  asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
+               ::"r"(tc::smem_u32(bar)), "h"((uint16_t)3) : "memory");
+}
+__device__ __forceinline__ void arrive_remote(uint32_t bar) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+
+// Descriptor of a 128-byte-swizzled operand tile as TMA writes it.
+//   K-major:  rows of 64 reduction steps (128 bytes), 1024 bytes from one group of 8 rows to the next; 16 steps are 32 bytes.
+//   MN-major: a piece is 64 rows of A (or B) wide and 64 steps tall, 128 bytes a step; 1024 bytes from 8 steps to the next 8,
+//             8192 from one piece to the next; 16 steps are 2048 bytes.
+template <bool MN> __device__ __forceinline__ uint64_t operand_desc(uint32_t addr) {
+  uint64_t d = (uint64_t)((addr >> 4) & 0x3FFFu);
+  d |= (uint64_t)((MN ? 8192u : 16u) >> 4) << 16;
+  d |= (uint64_t)(1024u >> 4) << 32;
+  d |= 1ull << 46;
+  d |= 2ull << 61;
+  return d;
+}
+template <bool MN> __host__ __device__ constexpr uint32_t operand_step() { return (MN ? 2048u : 32u) >> 4; }
+
+template <typename T> struct Format { static constexpr uint32_t code = 0; };                       // fp16
+template <> struct Format<__nv_bfloat16> { static constexpr uint32_t code = 1; };
+template <typename T> __host__ __device__ constexpr uint32_t idesc_of(bool a_mn, bool b_mn, uint32_t M, uint32_t N) {
+  return tc::instr_desc(Format<T>::code, M, N) | (a_mn ? 1u << 15 : 0u) | (b_mn ? 1u << 16 : 0u);
+}
+
+// ---------------------------------------------------------------- activation
+
+// act(a) and, where wanted, act'(a). Both are a times a logistic function: silu s(a), gelu's tanh form s(2 z) with
+// z = sqrt(2 / pi) (a + 0.044715 a^3). Beyond |a| = 16 the latter is 0 or 1 to 32 bits; z stops there so that a^3 stays finite.
+// The exponential and the reciprocal are the approximate instructions: 2^-21, against results of 11 bits at most.
+__device__ __forceinline__ float logistic(float x) { return __fdividef(1.f, 1.f + __expf(-x)); }
+template <bool Slope> __device__ __forceinline__ float activate(float a, int gelu, float& slope) {
+  if (gelu) {
+    const float c = 0.7978845608028654f, t = fminf(fmaxf(a, -16.f), 16.f), t2 = t * t;
+    const float s = logistic(2.f * c * t * fmaf(0.044715f, t2, 1.f));
+    if constexpr (Slope) slope = fmaf(2.f * c * t * s * (1.f - s), fmaf(3.f * 0.044715f, t2, 1.f), s);
+    return a * s;
+  }
+  const float s = logistic(a);
+  if constexpr (Slope) slope = s * fmaf(a, 1.f - s, 1.f);
+  return a * s;
+}
+
+// ---------------------------------------------------------------- the epilogue's chunks: 32 rows of 64 columns, swizzled
+
+template <typename T> __device__ __forceinline__ uint32_t pack2(float lo, float hi);
+template <> __device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi) {
+  const __half2 t = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&t);
+}
+template <> __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float lo, float hi) {
+  const __nv_bfloat162 t = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&t);
+}
+// 32 columns from `first` (0 or 32) of this lane's row
+template <typename T> __device__ __forceinline__ void put_row(char* chunk, int lane, int first, const float (&x)[32]) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    uint4 r;
+    r.x = pack2<T>(x[8 * j], x[8 * j + 1]); r.y = pack2<T>(x[8 * j + 2], x[8 * j + 3]);
+    r.z = pack2<T>(x[8 * j + 4], x[8 * j + 5]); r.w = pack2<T>(x[8 * j + 6], x[8 * j + 7]);
+    *reinterpret_cast<uint4*>(chunk + lane * 128 + (((first / 8 + j) ^ (lane & 7)) * 16)) = r;
+  }
+}
+template <typename T> __device__ __forceinline__ void get_row(const char* chunk, int lane, int first, float (&x)[32]) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const uint4 r = *reinterpret_cast<const uint4*>(chunk + lane * 128 + (((first / 8 + j) ^ (lane & 7)) * 16));
+    const T* e = reinterpret_cast<const T*>(&r);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[8 * j + i] = to_f32<T>(e[i]);
+  }
+}
+// A warp's chunk to rows row.., columns col.. of the result; what lies outside is dropped.
+template <typename T>
+__device__ __forceinline__ void store_chunk(const char* chunk, const CUtensorMap* map, T* plain, int64_t stride, int row, int col, int M,
+                                            int N, int lane) {
+  if (row >= M || col >= N) return;
+  if (plain == nullptr) {
+    tc::fence_async_smem();
+    __syncwarp();
+    if (lane == 0) {
+      tma_store(map, col, row, tc::smem_u32(chunk));
+      tc::bulk_commit();
+    }
+    return;
+  }
+  __syncwarp();
+  for (int r = 0; r < 32 && row + r < M; ++r)
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int c = lane + 32 * h;
+      const T e = *reinterpret_cast<const T*>(chunk + r * 128 + (((c >> 3) ^ (r & 7)) * 16) + (c & 7) * 2);
+      if (col + c < N) plain[(int64_t)(row + r) * stride + col + c] = e;
+    }
+}
+__device__ __forceinline__ void chunk_free(int lane) {        // the chunk may be written again
+  if (lane == 0) tc::bulk_wait_read_all();
+  __syncwarp();
+}
+
+// ---------------------------------------------------------------- tiles of 256 x 256
+
+struct Shared {
+  uint64_t full[8], empty[8], done[2], taken[2], loaded[kEpiWarps];
+  uint32_t tmem;
+  int abort;
+};
+
+// After a wait that ran out, copies and products of the block's own may still be on the way: they take microseconds, the block
+// stays two milliseconds before it gives up its memory. Called by every thread after a block barrier.
+__device__ __forceinline__ void after_a_failure(volatile int* abort) {
+  if (*abort) {
+    const long long t0 = clock64();
+    while (clock64() - t0 < 4000000) {}
+  }
+}
+
+// Tiles go in bands of 16 rows of tiles, down the rows first, so that the pairs at work at one time share operands in L2.
+__device__ __forceinline__ void tile_at(const Problem& p, int i, int& m, int& n) {
+  const int band = 16, per = band * p.tiles_n, b = i / per, rows = min(band, p.tiles_m - b * band);
+  m = b * band + (i - b * per) % rows;
+  n = (i - b * per) / rows;
+}
+
+template <typename T, int K, bool A_MN, bool B_MN>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
+product_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Problem p, uint32_t* status) {
+  constexpr int S = stages<K>();
+  extern __shared__ __align__(1024) char smem_raw[];
+  __shared__ Shared sh;
+  char* ring = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  char* staging = ring + S * kStageBytes;
+  const int tid = threadIdx.x, lane = tid & 31, wid = tid >> 5;
+  const uint32_t rank = cluster_rank();
+  const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+  const int tiles = p.tiles_m * p.tiles_n, steps = p.steps[0] + p.steps[1];
+
+  if (wid == 0 && lane == 0) {
+    for (int i = 0; i < S; ++i) {
+      tc::mbar_init(&sh.full[i], 1);
+      tc::mbar_init(&sh.empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      tc::mbar_init(&sh.done[i], 1);
+      tc::mbar_init(&sh.taken[i], 2 * kEpiWarps);
+    }
+    for (int i = 0; i < kEpiWarps; ++i) tc::mbar_init(&sh.loaded[i], 1);
+    sh.abort = 0;
+    tc::mbar_init_fence();
+  }
+  if (wid == 2) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tc::smem_u32(&sh.tmem)), "r"(512u) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  }
+  tc::tc_fence_before_sync();
+  __syncthreads();
+  cluster_sync();
+  tc::tc_fence_after_sync();
+  const uint32_t tmem = sh.tmem;
+
+  if (wid == 0) {
+    // ---- copies: this block's rows of A and its half of B, counted on block 0's barrier
+    if (lane == 0) {
+      int s = 0, phase = 0;
+      bool ok = true;
+      for (int i = pair; ok && i < tiles; i += pairs) {
+        int m, n;
+        tile_at(p, i, m, n);
+        const bool lower = p.split_m > 0 && m >= p.split_m;
+        const int row_a = (lower ? m - p.split_m : m) * kTile + rank * kBlockRows;
+        const int row_b = K == kGated ? n * kBlockRows : n * kTile + (int)rank * kBlockRows;
+        for (int k = 0; k < steps; ++k) {
+          const int run = k >= p.steps[0], at = (run ? k - p.steps[0] : k) * kStep;
+          const CUtensorMap* ma = &maps.a[lower || run ? 1 : 0];
+          const CUtensorMap* mb = &maps.b[K == kGated ? (int)rank : run];
+          if (!tc::mbar_wait(&sh.empty[s], phase ^ 1, &sh.abort, status, kWaitCode)) { ok = false; break; }
+          const uint32_t bar = in_block(tc::smem_u32(&sh.full[s]), 0), dst = tc::smem_u32(ring + s * kStageBytes);
+          if (rank == 0) tc::mbar_expect_tx(&sh.full[s], 2 * kStageBytes);
+          if constexpr (A_MN) {
+            tma_load_pair(dst, ma, row_a, at, bar);
+            tma_load_pair(dst + kOperandBytes / 2, ma, row_a + 64, at, bar);
+          } else {
+            tma_load_pair(dst, ma, at, row_a, bar);
+          }
+          if constexpr (B_MN) {
+            tma_load_pair(dst + kOperandBytes, mb, row_b, at, bar);
+            tma_load_pair(dst + kOperandBytes + kOperandBytes / 2, mb, row_b + 64, at, bar);
+          } else {
+            tma_load_pair(dst + kOperandBytes, mb, at, row_b, bar);
+          }
+          if (++s == S) { s = 0; phase ^= 1; }
+        }
+      }
+    }
+    __syncwarp();
+  } else if (wid == 1) {
+    // ---- products: one thread of block 0 for both
+    if (rank == 0 && lane == 0) {
+      constexpr uint32_t idesc = idesc_of<T>(A_MN, B_MN, kTile, kTile);
+      int s = 0, phase = 0, buf = 0, taken = 1;
+      bool ok = true;
+      for (int i = pair; ok && i < tiles; i += pairs) {
+        if (!tc::mbar_wait(&sh.taken[buf], taken, &sh.abort, status, kWaitCode)) break;
+        tc::tc_fence_after_sync();
+        const uint32_t d = tmem + buf * kTile;
+        for (int k = 0; k < steps; ++k) {
+          if (!tc::mbar_wait(&sh.full[s], phase, &sh.abort, status, kWaitCode)) { ok = false; break; }
+          tc::tc_fence_after_sync();
+          const uint32_t at = tc::smem_u32(ring + s * kStageBytes);
+          uint64_t a = operand_desc<A_MN>(at), b = operand_desc<B_MN>(at + kOperandBytes);
+#pragma unroll
+          for (int q = 0; q < kStep / 16; ++q)
+            mma_pair(d, a + q * operand_step<A_MN>(), b + q * operand_step<B_MN>(), idesc, (k | q) != 0);
+          commit_pair(&sh.empty[s]);
+          if (++s == S) { s = 0; phase ^= 1; }
+        }
+        if (ok) commit_pair(&sh.done[buf]);
+        if (buf == 1) taken ^= 1;
+        buf ^= 1;
+      }
+    }
+    __syncwarp();
+  } else if (wid >= 4) {
+    // ---- results: lanes 32 (wid % 4).. of tensor memory, the first or the second half of the columns
+    const int quad = wid & 3, half = (wid - 4) >> 2, ew = wid - 4;
+    char* chunk = staging + ew * (staging_bytes<K>() / kEpiWarps);
+    const uint32_t lanes = (uint32_t)(quad * 32) << 16;
+    const uint32_t taken0 = in_block(tc::smem_u32(&sh.taken[0]), 0), taken1 = in_block(tc::smem_u32(&sh.taken[1]), 0);
+    int buf = 0, phase = 0;
+    int loads = 0;                                    // kGatedBackward: chunks loaded so far
+    auto load_chunk = [&](int i, int c) {             // chunk c (0, 1) of this warp's half of tile i: a and u
+      if (i >= tiles) return;
+      int m, n;
+      tile_at(p, i, m, n);
+      if (lane == 0) {
+        const int row = m * kTile + rank * kBlockRows + quad * 32, col = n * kTile + half * 128 + c * kChunk16;
+        tc::mbar_expect_tx(&sh.loaded[ew], 2 * kChunkBytes);
+        tma_load(tc::smem_u32(chunk), &maps.in[0], col, row, tc::smem_u32(&sh.loaded[ew]));
+        tma_load(tc::smem_u32(chunk + kChunkBytes), &maps.in[1], col, row, tc::smem_u32(&sh.loaded[ew]));
+      }
+    };
+    if constexpr (K == kGatedBackward) load_chunk(pair, 0);
+    for (int i = pair; i < tiles; i += pairs) {
+      int m, n;
+      tile_at(p, i, m, n);
+      const bool lower = p.split_m > 0 && m >= p.split_m;
+      const int row = (lower ? m - p.split_m : m) * kTile + rank * kBlockRows + quad * 32;
+      if (!tc::mbar_wait_warp(&sh.done[buf], phase, &sh.abort, status, kWaitCode)) break;
+      tc::tc_fence_after_sync();
+      const uint32_t acc = tmem + lanes + buf * kTile;
+      if constexpr (K == kPlain) {
+        const CUtensorMap* map = &maps.out[lower];
+        T* plain = static_cast<T*>(p.plain_out[lower]);
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          const int at = half * 128 + c * kChunk16;
+          float x[32];
+          chunk_free(lane);
+#pragma unroll
+          for (int q = 0; q < 2; ++q) {
+            tc::tmem_ld32(acc + at + 32 * q, x);
+            tc::tmem_ld_wait();
+            put_row<T>(chunk, lane, 32 * q, x);
+          }
+          store_chunk<T>(chunk, map, plain, p.out_stride, row, n * kTile + at, p.M, p.N, lane);
+          if (plain) __syncwarp();
+        }
+      } else if constexpr (K == kGated) {
+        const int col = n * kBlockRows + half * kChunk16;
+        uint32_t a16[32], u16[32];                    // a and u as they are kept, in pairs
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+          float a[32], u[32];
+          tc::tmem_ld32(acc + half * kChunk16 + 32 * q, a);
+          tc::tmem_ld32(acc + kBlockRows + half * kChunk16 + 32 * q, u);
+          tc::tmem_ld_wait();
+          if (p.save) {
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+              a16[16 * q + j] = pack2<T>(a[2 * j], a[2 * j + 1]);
+              u16[16 * q + j] = pack2<T>(u[2 * j], u[2 * j + 1]);
+            }
+          }
+#pragma unroll
+          for (int j = 0; j < 32; ++j) {
+            float none;
+            a[j] = activate<false>(a[j], p.gelu, none) * u[j];
+          }
+          if (q == 0) chunk_free(lane);
+          put_row<T>(chunk, lane, 32 * q, a);
+        }
+        store_chunk<T>(chunk, &maps.out[0], nullptr, 0, row, col, p.M, p.N, lane);
+        if (p.save) {
+#pragma unroll
+          for (int part = 0; part < 2; ++part) {
+            chunk_free(lane);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              const uint32_t* w = part ? u16 : a16;
+              *reinterpret_cast<uint4*>(chunk + lane * 128 + ((j ^ (lane & 7)) * 16)) =
+                  make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
+            }
+            store_chunk<T>(chunk, &maps.out[1 + part], nullptr, 0, row, col, p.M, p.N, lane);
+          }
+        }
+      } else {
+        bool ok = true;
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          const int at = half * 128 + c * kChunk16;
+          ok = tc::mbar_wait_warp(&sh.loaded[ew], loads & 1, &sh.abort, status, kWaitCode);
+          if (!ok) break;
+          ++loads;
+#pragma unroll
+          for (int q = 0; q < 2; ++q) {
+            float d[32], a[32], u[32];
+            tc::tmem_ld32(acc + at + 32 * q, d);
+            get_row<T>(chunk, lane, 32 * q, a);
+            get_row<T>(chunk + kChunkBytes, lane, 32 * q, u);
+            tc::tmem_ld_wait();
+#pragma unroll
+            for (int j = 0; j < 32; ++j) {
+              float slope;
+              const float act = activate<true>(a[j], p.gelu, slope);
+              a[j] = d[j] * u[j] * slope;
+              u[j] = d[j] * act;
+            }
+            put_row<T>(chunk, lane, 32 * q, a);
+            put_row<T>(chunk + kChunkBytes, lane, 32 * q, u);
+          }
+          store_chunk<T>(chunk, &maps.out[0], nullptr, 0, row, n * kTile + at, p.M, p.N, lane);
+          store_chunk<T>(chunk + kChunkBytes, &maps.out[1], nullptr, 0, row, n * kTile + at, p.M, p.N, lane);
+          tc::fence_async_smem();                     // a chunk outside the result was not stored: order its rewriting all the same
+          chunk_free(lane);
+          if (c == 0) load_chunk(i, 1); else load_chunk(i + pairs, 0);
+        }
+        if (!ok) break;
+      }
+      tc::tc_fence_before_sync();
+      __syncwarp();
+      if (lane == 0) arrive_remote(buf ? taken1 : taken0);
+      if (buf == 1) phase ^= 1;
+      buf ^= 1;
+    }
+    if (lane == 0) tc::bulk_wait_all();               // nothing reads this block's memory any more
+    __syncwarp();
+  }
+  __syncthreads();
+  after_a_failure(&sh.abort);
+  cluster_sync();                                     // neither block leaves while the other's products or copies need it
+  if (wid == 2)
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+}
+
+// ---------------------------------------------------------------- few tokens
+
+constexpr int kSkinnyThreads = 256;
+constexpr int kMaxSplit = 8;
+constexpr int kSkinnyTokens = 64;                // the most tokens of a call that goes this way
+
+struct __align__(64) SkinnyMaps {
+  CUtensorMap w[2], x;                           // weights (Wg, Wu; or Wd alone) in boxes of 128 rows, tokens in boxes of `width`
+};
+struct Skinny {
+  int steps;                                     // stages of the whole reduction
+  int stages, stage_bytes;
+  int tokens, width;                             // width: tokens rounded up to 16
+  int rows;                                      // weight rows: inner channels, or outputs
+  int gelu;
+  void *out, *a, *u;                             // a, u: kept for a backward pass, or null
+  int64_t out_stride, au_stride;
+};
+
+template <typename T, bool Gated>
+__global__ void __launch_bounds__(kSkinnyThreads, 1) skinny_kernel(const __grid_constant__ SkinnyMaps maps, const __grid_constant__ Skinny p,
+                                                                  uint32_t* status) {
+  extern __shared__ __align__(1024) char smem_raw[];
+  __shared__ Shared sh;
+  char* ring = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  const int tid = threadIdx.x, lane = tid & 31, wid = tid >> 5;
+  const int rank = (int)cluster_rank(), CL = (int)gridDim.y;      // the cluster lies along y
+  const int row0 = blockIdx.x * kBlockRows;
+  const int k0 = (int)((int64_t)p.steps * rank / CL), k1 = (int)((int64_t)p.steps * (rank + 1) / CL);
+  constexpr int kWeightBytes = (Gated ? 2 : 1) * kOperandBytes;
+  const int token_bytes = p.width * kStep * 2;
+  if (wid == 0 && lane == 0) {
+    for (int i = 0; i < p.stages; ++i) {
+      tc::mbar_init(&sh.full[i], 1);
+      tc::mbar_init(&sh.empty[i], 1);
+    }
+    tc::mbar_init(&sh.done[0], 1);
+    sh.abort = 0;
+    tc::mbar_init_fence();
+  }
+  if (wid == 2) tc::tmem_alloc(&sh.tmem, 128);
+  tc::tc_fence_before_sync();
+  __syncthreads();
+  tc::tc_fence_after_sync();
+  const uint32_t tmem = sh.tmem;
+
+  if (wid == 0) {
+    if (lane == 0) {
+      int s = 0, phase = 0;
+      for (int k = k0; k < k1; ++k) {
+        if (!tc::mbar_wait(&sh.empty[s], phase ^ 1, &sh.abort, status, kWaitCode)) break;
+        const uint32_t bar = tc::smem_u32(&sh.full[s]), dst = tc::smem_u32(ring + s * p.stage_bytes);
+        tc::mbar_expect_tx(&sh.full[s], kWeightBytes + token_bytes);
+        tma_load(dst, &maps.w[0], k * kStep, row0, bar);
+        if constexpr (Gated) tma_load(dst + kOperandBytes, &maps.w[1], k * kStep, row0, bar);
+        tma_load(dst + kWeightBytes, &maps.x, k * kStep, 0, bar);
+        if (++s == p.stages) { s = 0; phase ^= 1; }
+      }
+    }
+    __syncwarp();
+  } else if (wid == 1) {
+    if (lane == 0) {
+      const uint32_t idesc = idesc_of<T>(false, false, kBlockRows, p.width);
+      int s = 0, phase = 0;
+      bool ok = true;
+      for (int k = k0; k < k1; ++k) {
+        if (!tc::mbar_wait(&sh.full[s], phase, &sh.abort, status, kWaitCode)) { ok = false; break; }
+        tc::tc_fence_after_sync();
+        const uint32_t at = tc::smem_u32(ring + s * p.stage_bytes);
+        const uint64_t w = operand_desc<false>(at), x = operand_desc<false>(at + kWeightBytes);
+#pragma unroll
+        for (int q = 0; q < kStep / 16; ++q) {
+          const uint32_t acc = k > k0 || q > 0;
+          tc::mma_bf16(tmem, w + q * operand_step<false>(), x + q * operand_step<false>(), idesc, acc);
+          if constexpr (Gated)
+            tc::mma_bf16(tmem + 64, w + (kOperandBytes >> 4) + q * operand_step<false>(), x + q * operand_step<false>(), idesc, acc);
+        }
+        tc::mma_commit(&sh.empty[s]);
+        if (++s == p.stages) { s = 0; phase ^= 1; }
+      }
+      if (ok) tc::mma_commit(&sh.done[0]);
+    }
+    __syncwarp();
+  } else if (wid >= 4) {
+    // partial sums to this block's shared memory, [gate | up][token][weight row]; the ring is free: every product has read it
+    const int quad = wid & 3;
+    float* part = reinterpret_cast<float*>(ring);
+    if (tc::mbar_wait_warp(&sh.done[0], 0, &sh.abort, status, kWaitCode)) {
+      tc::tc_fence_after_sync();
+      for (int n = 0; n < p.width; n += 16) {
+#pragma unroll
+        for (int g = 0; g < (Gated ? 2 : 1); ++g) {
+          float x[16];
+          tc::tmem_ld16(tmem + ((uint32_t)(quad * 32) << 16) + g * 64 + n, x);
+          tc::tmem_ld_wait();
+#pragma unroll
+          for (int j = 0; j < 16; ++j) part[(g * p.width + n + j) * kBlockRows + quad * 32 + lane] = x[j];
+        }
+      }
+      tc::tc_fence_before_sync();
+    }
+  }
+  __syncthreads();
+  after_a_failure(&sh.abort);
+  if (CL > 1) cluster_sync();
+  // every block finishes the tokens n = rank, rank + CL, ...: a thread a weight row, the blocks' sums in their order
+  {
+    const int r = tid & (kBlockRows - 1), row = row0 + r;
+    const uint32_t part = tc::smem_u32(ring);
+    if (row < p.rows)
+      for (int n = rank + CL * (tid / kBlockRows); n < p.tokens; n += CL * (kSkinnyThreads / kBlockRows)) {
+        float v[2] = {0.f, 0.f};
+        for (int b = 0; b < CL; ++b) {
+          const uint32_t peer = CL > 1 ? in_block(part, b) : part;
+#pragma unroll
+          for (int g = 0; g < (Gated ? 2 : 1); ++g) {
+            float x;
+            asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(x) : "r"(peer + ((g * p.width + n) * kBlockRows + r) * 4) : "memory");
+            v[g] += x;
+          }
+        }
+        T* out = static_cast<T*>(p.out) + (int64_t)n * p.out_stride + row;
+        if constexpr (Gated) {
+          float none;
+          *out = from_f32<T>(activate<false>(v[0], p.gelu, none) * v[1]);
+          if (p.a) {
+            static_cast<T*>(p.a)[(int64_t)n * p.au_stride + row] = from_f32<T>(v[0]);
+            static_cast<T*>(p.u)[(int64_t)n * p.au_stride + row] = from_f32<T>(v[1]);
+          }
+        } else {
+          *out = from_f32<T>(v[0]);
+        }
+      }
+  }
+  __syncthreads();
+  if (CL > 1) cluster_sync();                         // no block leaves while another reads its sums
+  if (wid == 2) tc::tmem_dealloc(tmem, 128);
+}
+
+// ---------------------------------------------------------------- rows to a pitch of 16 bytes
+
+constexpr int kMaxCopies = 6;
+struct Copies {
+  const uint16_t* src[kMaxCopies];
+  uint16_t* dst[kMaxCopies];
+  int64_t rows[kMaxCopies], src_stride[kMaxCopies], dst_stride[kMaxCopies];
+  int cols[kMaxCopies];
+};
+// 8 elements a thread; what lies behind a row's end is zero
+__global__ void __launch_bounds__(256) align_rows_kernel(const __grid_constant__ Copies c) {
+  const int j = blockIdx.y, per = (c.cols[j] + 7) / 8;
+  const int64_t n = c.rows[j] * per;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
+    const int64_t r = i / per;
+    const int at = (int)(i - r * per) * 8;
+    const uint16_t* s = c.src[j] + r * c.src_stride[j] + at;
+    uint16_t e[8];
+#pragma unroll
+    for (int q = 0; q < 8; ++q) e[q] = at + q < c.cols[j] ? s[q] : (uint16_t)0;
+    *reinterpret_cast<uint4*>(c.dst[j] + r * c.dst_stride[j] + at) = *reinterpret_cast<const uint4*>(e);
+  }
+}
+
+// ---------------------------------------------------------------- host side
+
+using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                                 const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                 CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeTiled encode_tiled() {
+  static const EncodeTiled fn = [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &p, 12000, cudaEnableDefault, &q) != cudaSuccess ||
+        q != cudaDriverEntryPointSuccess)
+      p = nullptr;
+    return reinterpret_cast<EncodeTiled>(p);
+  }();
+  return fn;
+}
+
+// a [rows, cols] matrix of 16-bit elements with rows `stride` elements apart, in boxes of box_rows x 64
+struct Matrix {
+  const void* p;
+  int64_t rows, cols, stride;
+};
+bool make_map(CUtensorMap* map, const Matrix& m, int box_rows, int dtype) {
+  const EncodeTiled fn = encode_tiled();
+  if (!fn) return false;
+  const cuuint64_t dims[2] = {(cuuint64_t)m.cols, (cuuint64_t)m.rows}, strides[1] = {(cuuint64_t)m.stride * 2};
+  const cuuint32_t box[2] = {64, (cuuint32_t)box_rows}, unit[2] = {1, 1};
+  return fn(map, dtype == GDN2_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, const_cast<void*>(m.p), dims,
+            strides, box, unit, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// Encoding a map is a driver call that needs the device's context to be the thread's own, which a thread that has made no runtime
+// call yet (an autograd engine's) lacks.
+int own_context() {
+  int dev = 0;
+  GDN2_CUDA_TRY(cudaGetDevice(&dev));
+  GDN2_CUDA_TRY(cudaSetDevice(dev));
+  return GDN2_OK;
+}
+
+bool aligned_rows(const Matrix& m) { return (reinterpret_cast<uintptr_t>(m.p) & 15u) == 0 && m.stride % 8 == 0; }
+int steps_of(int64_t k) { return (int)((k + kStep - 1) / kStep); }
+int tiles_of(int64_t n, int tile) { return (int)((n + tile - 1) / tile); }
+
+template <typename T, int K, bool A_MN, bool B_MN>
+int launch_product(const Maps& maps, const Problem& p, cudaStream_t st) {
+  uint32_t* status = device_status_word();
+  if (!status) return record_cuda_error(cudaGetLastError());
+  auto kernel = product_kernel<T, K, A_MN, B_MN>;
+  GDN2_CUDA_TRY(ensure_dynamic_smem(reinterpret_cast<const void*>(kernel), smem_bytes<K>()));
+  const int tiles = p.tiles_m * p.tiles_n, pairs = device_sm_count() / 2;
+  kernel<<<2 * (tiles < pairs ? tiles : pairs), kThreads, smem_bytes<K>(), st>>>(maps, p, status);
+  GDN2_CUDA_TRY(cudaGetLastError());
+  return GDN2_OK;
+}
+
+#define GDN2_MAP(m, matrix, box)                                     \
+  do {                                                               \
+    if (!make_map(&(m), matrix, box, dtype)) return GDN2_ERR_UNSUPPORTED; \
+  } while (0)
+
+// h (and a, u) = the gated product of x and Wg, Wu
+template <typename T>
+int gated_forward(const Matrix& x, const Matrix& wg, const Matrix& wu, const Matrix& h, const Matrix* a, const Matrix* u, int gelu, int dtype,
+                  cudaStream_t st) {
+  Maps maps{};
+  Problem p{};
+  GDN2_MAP(maps.a[0], x, kBlockRows);
+  GDN2_MAP(maps.b[0], wg, kBlockRows);
+  GDN2_MAP(maps.b[1], wu, kBlockRows);
+  GDN2_MAP(maps.out[0], h, 32);
+  if (a) {
+    GDN2_MAP(maps.out[1], *a, 32);
+    GDN2_MAP(maps.out[2], *u, 32);
+  }
+  p.steps[0] = steps_of(x.cols);
+  p.tiles_m = tiles_of(x.rows, kTile);
+  p.tiles_n = tiles_of(wg.rows, kBlockRows);
+  p.M = (int)x.rows;
+  p.N = (int)wg.rows;
+  p.save = a != nullptr;
+  p.gelu = gelu;
+  return launch_product<T, kGated, false, false>(maps, p, st);
+}
+
+// da, du from dy, Wd and the kept a, u
+template <typename T>
+int gated_backward(const Matrix& dy, const Matrix& wd, const Matrix& a, const Matrix& u, const Matrix& da, const Matrix& du, int gelu,
+                   int dtype, cudaStream_t st) {
+  Maps maps{};
+  Problem p{};
+  GDN2_MAP(maps.a[0], dy, kBlockRows);
+  GDN2_MAP(maps.b[0], wd, kStep);
+  GDN2_MAP(maps.in[0], a, 32);
+  GDN2_MAP(maps.in[1], u, 32);
+  GDN2_MAP(maps.out[0], da, 32);
+  GDN2_MAP(maps.out[1], du, 32);
+  p.steps[0] = steps_of(dy.cols);
+  p.tiles_m = tiles_of(dy.rows, kTile);
+  p.tiles_n = tiles_of(wd.cols, kTile);
+  p.M = (int)dy.rows;
+  p.N = (int)wd.cols;
+  p.gelu = gelu;
+  return launch_product<T, kGatedBackward, false, true>(maps, p, st);
+}
+
+int set_out(Maps& maps, Problem& p, int part, const Matrix& out, int dtype) {
+  p.out_stride = out.stride;
+  if (aligned_rows(out)) GDN2_MAP(maps.out[part], out, 32);
+  else p.plain_out[part] = const_cast<void*>(out.p);
+  return GDN2_OK;
+}
+
+// out [M, N] = sum over the runs of a_i b_i^T, the operands as they lie: a [M, K] (or [K, M]), b [N, K] (or [K, N])
+template <typename T, bool A_MN, bool B_MN>
+int product(const Matrix* a, const Matrix* b, int runs, const Matrix& out, int dtype, cudaStream_t st) {
+  Maps maps{};
+  Problem p{};
+  for (int i = 0; i < runs; ++i) {
+    GDN2_MAP(maps.a[i], a[i], A_MN ? kStep : kBlockRows);
+    GDN2_MAP(maps.b[i], b[i], B_MN ? kStep : kBlockRows);
+    p.steps[i] = steps_of(A_MN ? a[i].rows : a[i].cols);
+  }
+  const int rc = set_out(maps, p, 0, out, dtype);
+  if (rc != GDN2_OK) return rc;
+  p.tiles_m = tiles_of(out.rows, kTile);
+  p.tiles_n = tiles_of(out.cols, kTile);
+  p.M = (int)out.rows;
+  p.N = (int)out.cols;
+  return launch_product<T, kPlain, A_MN, B_MN>(maps, p, st);
+}
+// out_i [M, N] = a_i^T b for two a [K, M] and one b [K, N], in one launch
+template <typename T>
+int two_weight_gradients(const Matrix& a0, const Matrix& a1, const Matrix& b, const Matrix& out0, const Matrix& out1, int dtype, cudaStream_t st) {
+  Maps maps{};
+  Problem p{};
+  GDN2_MAP(maps.a[0], a0, kStep);
+  GDN2_MAP(maps.a[1], a1, kStep);
+  GDN2_MAP(maps.b[0], b, kStep);
+  int rc = set_out(maps, p, 0, out0, dtype);
+  if (rc == GDN2_OK) rc = set_out(maps, p, 1, out1, dtype);
+  if (rc != GDN2_OK) return rc;
+  p.steps[0] = steps_of(b.rows);
+  p.split_m = tiles_of(out0.rows, kTile);
+  p.tiles_m = 2 * p.split_m;
+  p.tiles_n = tiles_of(out0.cols, kTile);
+  p.M = (int)out0.rows;
+  p.N = (int)out0.cols;
+  return launch_product<T, kPlain, true, true>(maps, p, st);
+}
+
+template <typename T, bool Gated>
+int launch_skinny(const Matrix& x, const Matrix& w0, const Matrix* w1, const Matrix& out, void* a, void* u, int64_t au_stride, int gelu,
+                  int dtype, cudaStream_t st) {
+  SkinnyMaps maps{};
+  Skinny p{};
+  p.tokens = (int)x.rows;
+  p.width = (p.tokens + 15) / 16 * 16;
+  GDN2_MAP(maps.w[0], w0, kBlockRows);
+  if (w1) GDN2_MAP(maps.w[1], *w1, kBlockRows);
+  GDN2_MAP(maps.x, x, p.width);
+  p.steps = steps_of(x.cols);
+  p.rows = (int)w0.rows;
+  p.gelu = gelu;
+  p.out = const_cast<void*>(out.p);
+  p.out_stride = out.stride;
+  p.a = a; p.u = u; p.au_stride = au_stride;
+  p.stage_bytes = (Gated ? 2 : 1) * kOperandBytes + p.width * kStep * 2;
+  p.stages = (220 * 1024) / p.stage_bytes;
+  if (p.stages > 8) p.stages = 8;
+  size_t smem = (size_t)p.stages * p.stage_bytes + 1024;
+  const size_t sums = (size_t)(Gated ? 2 : 1) * p.width * kBlockRows * 4 + 1024;
+  if (smem < sums) smem = sums;
+  // as many blocks a tile as it takes to give every SM one, each with two stages of the reduction at least
+  const int tiles = tiles_of(w0.rows, kBlockRows);
+  int split = device_sm_count() / tiles;
+  if (split > kMaxSplit) split = kMaxSplit;
+  if (split > p.steps / 2) split = p.steps / 2;
+  if (split < 1) split = 1;
+  uint32_t* status = device_status_word();
+  if (!status) return record_cuda_error(cudaGetLastError());
+  auto kernel = skinny_kernel<T, Gated>;
+  GDN2_CUDA_TRY(ensure_dynamic_smem(reinterpret_cast<const void*>(kernel), 224 * 1024));
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 1;
+  attr[0].val.clusterDim.y = split;
+  attr[0].val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(tiles, split);
+  cfg.blockDim = dim3(kSkinnyThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  GDN2_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, maps, p, status));
+  return GDN2_OK;
+}
+
+template <typename T> int forward(const gdn2_ffn_args& f, int dtype, cudaStream_t st) {
+  const Matrix x{f.x, f.tokens, f.hidden, f.x_stride}, wg{f.w_gate, f.inner, f.hidden, f.w_gate_stride},
+      wu{f.w_up, f.inner, f.hidden, f.w_up_stride}, wd{f.w_down, f.out, f.inner, f.w_down_stride}, h{f.h, f.tokens, f.inner, f.inner_stride},
+      y{f.y, f.tokens, f.out, f.y_stride}, a{f.a, f.tokens, f.inner, f.inner_stride}, u{f.u, f.tokens, f.inner, f.inner_stride};
+  const int gelu = f.activation == GDN2_ACT_GELU_TANH;
+  int rc;
+  if (f.tokens <= kSkinnyTokens) {
+    rc = launch_skinny<T, true>(x, wg, &wu, h, f.a, f.u, f.inner_stride, gelu, dtype, st);
+    if (rc != GDN2_OK) return rc;
+    return launch_skinny<T, false>(h, wd, nullptr, y, nullptr, nullptr, 0, 0, dtype, st);
+  }
+  rc = gated_forward<T>(x, wg, wu, h, f.a ? &a : nullptr, &u, gelu, dtype, st);
+  if (rc != GDN2_OK) return rc;
+  return product<T, false, false>(&h, &wd, 1, y, dtype, st);
+}
+
+template <typename T> int backward(const gdn2_ffn_args& f, int dtype, cudaStream_t st) {
+  const Matrix x{f.x, f.tokens, f.hidden, f.x_stride}, wg{f.w_gate, f.inner, f.hidden, f.w_gate_stride},
+      wu{f.w_up, f.inner, f.hidden, f.w_up_stride}, wd{f.w_down, f.out, f.inner, f.w_down_stride}, h{f.h, f.tokens, f.inner, f.inner_stride},
+      a{f.a, f.tokens, f.inner, f.inner_stride}, u{f.u, f.tokens, f.inner, f.inner_stride}, dy{f.dy, f.tokens, f.out, f.dy_stride},
+      da{f.da, f.tokens, f.inner, f.inner_stride}, du{f.du, f.tokens, f.inner, f.inner_stride}, dx{f.dx, f.tokens, f.hidden, f.dx_stride},
+      dwg{f.dw_gate, f.inner, f.hidden, f.hidden}, dwu{f.dw_up, f.inner, f.hidden, f.hidden}, dwd{f.dw_down, f.out, f.inner, f.inner};
+  int rc = GDN2_OK;
+  if (f.dx || f.dw_gate) rc = gated_backward<T>(dy, wd, a, u, da, du, f.activation == GDN2_ACT_GELU_TANH, dtype, st);
+  if (rc == GDN2_OK && f.dx) {
+    const Matrix lhs[2] = {da, du}, rhs[2] = {wg, wu};
+    rc = product<T, false, true>(lhs, rhs, 2, dx, dtype, st);
+  }
+  if (rc == GDN2_OK && f.dw_gate) rc = two_weight_gradients<T>(da, du, x, dwg, dwu, dtype, st);
+  if (rc == GDN2_OK && f.dw_down) rc = product<T, true, true>(&dy, &h, 1, dwd, dtype, st);
+  return rc;
+}
+
+int check(const gdn2_ffn_args& f, int dtype, bool back) {
+  if (dtype != GDN2_BF16 && dtype != GDN2_F16) return GDN2_ERR_BAD_DTYPE;
+  if (f.activation != GDN2_ACT_SILU && f.activation != GDN2_ACT_GELU_TANH) return GDN2_ERR_UNSUPPORTED;
+  const int64_t most = 1LL << 30;
+  for (int64_t n : {f.tokens, f.hidden, f.inner, f.out})
+    if (n <= 0 || n > most) return GDN2_ERR_BAD_SHAPE;
+  // tiles are counted in 32 bits
+  if (((f.tokens >> 7) + 1) * ((f.inner >> 6) + 1) > most || ((f.inner >> 7) + 1) * ((f.hidden >> 6) + 1) > most ||
+      ((f.tokens >> 7) + 1) * ((f.out >> 6) + 1) > most || ((f.tokens >> 7) + 1) * ((f.hidden >> 6) + 1) > most ||
+      ((f.out >> 7) + 1) * ((f.inner >> 6) + 1) > most)
+    return GDN2_ERR_BAD_SHAPE;
+  if (!f.x || !f.w_gate || !f.w_up || !f.w_down || !f.h) return GDN2_ERR_NULL_POINTER;
+  if (back) {
+    if (!f.dy || !f.a || !f.u) return GDN2_ERR_NULL_POINTER;
+    if ((f.dx || f.dw_gate) && (!f.da || !f.du)) return GDN2_ERR_NULL_POINTER;
+    if ((f.dw_gate == nullptr) != (f.dw_up == nullptr)) return GDN2_ERR_NULL_POINTER;
+  } else {
+    if (!f.y || (f.a == nullptr) != (f.u == nullptr)) return GDN2_ERR_NULL_POINTER;
+  }
+  if (f.x_stride < f.hidden || f.w_gate_stride < f.hidden || f.w_up_stride < f.hidden || f.w_down_stride < f.inner ||
+      f.inner_stride < f.inner || (back ? f.dy_stride < f.out || (f.dx && f.dx_stride < f.hidden) : f.y_stride < f.out))
+    return GDN2_ERR_BAD_SHAPE;
+  for (int64_t s : {f.x_stride, f.w_gate_stride, f.w_up_stride, f.w_down_stride, f.inner_stride, back ? f.dy_stride : (int64_t)0})
+    if (s % 8 || s > (1LL << 34)) return GDN2_ERR_MISALIGNED;
+  for (const void* q : {f.x, f.w_gate, f.w_up, f.w_down, (const void*)f.h, (const void*)f.a, (const void*)f.u, back ? f.dy : nullptr,
+                        back ? (const void*)f.da : nullptr, back ? (const void*)f.du : nullptr})
+    if (reinterpret_cast<uintptr_t>(q) & 15u) return GDN2_ERR_MISALIGNED;
+  return GDN2_OK;
+}
+
+}  // namespace
+}  // namespace gdn2
+
+extern "C" {
+
+int gdn2_ffn_forward(const gdn2_ffn_args* args, int dtype, void* stream) {
+  if (!args) return GDN2_ERR_NULL_POINTER;
+  int rc = gdn2::check(*args, dtype, false);
+  if (rc == GDN2_OK) rc = gdn2::own_context();
+  if (rc != GDN2_OK) return rc;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  return dtype == GDN2_BF16 ? gdn2::forward<__nv_bfloat16>(*args, dtype, st) : gdn2::forward<__half>(*args, dtype, st);
+}
+
+int gdn2_ffn_backward(const gdn2_ffn_args* args, int dtype, void* stream) {
+  if (!args) return GDN2_ERR_NULL_POINTER;
+  int rc = gdn2::check(*args, dtype, true);
+  if (rc == GDN2_OK) rc = gdn2::own_context();
+  if (rc != GDN2_OK) return rc;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  return dtype == GDN2_BF16 ? gdn2::backward<__nv_bfloat16>(*args, dtype, st) : gdn2::backward<__half>(*args, dtype, st);
+}
+
+int gdn2_align_rows(const gdn2_row_copy* copies, int64_t n, void* stream) {
+  using namespace gdn2;
+  if (!copies) return GDN2_ERR_NULL_POINTER;
+  if (n < 1 || n > kMaxCopies) return GDN2_ERR_BAD_SHAPE;
+  Copies c{};
+  int64_t most = 0;
+  for (int i = 0; i < n; ++i) {
+    const gdn2_row_copy& k = copies[i];
+    if (!k.src || !k.dst) return GDN2_ERR_NULL_POINTER;
+    if (k.rows < 1 || k.cols < 1 || k.cols > (1LL << 30) || k.rows > (1LL << 30) || k.dst_stride < k.cols || k.src_stride < 0)
+      return GDN2_ERR_BAD_SHAPE;
+    if ((reinterpret_cast<uintptr_t>(k.dst) & 15u) || k.dst_stride % 8) return GDN2_ERR_MISALIGNED;
+    c.src[i] = static_cast<const uint16_t*>(k.src);
+    c.dst[i] = static_cast<uint16_t*>(k.dst);
+    c.rows[i] = k.rows; c.cols[i] = (int)k.cols; c.src_stride[i] = k.src_stride; c.dst_stride[i] = k.dst_stride;
+    const int64_t pieces = k.rows * ((k.cols + 7) / 8);
+    most = pieces > most ? pieces : most;
+  }
+  const int64_t blocks = (most + 255) / 256, cap = 8LL * device_sm_count();
+  align_rows_kernel<<<dim3((unsigned)(blocks < cap ? blocks : cap), (unsigned)n), 256, 0, static_cast<cudaStream_t>(stream)>>>(c);
+  GDN2_CUDA_TRY(cudaGetLastError());
+  return GDN2_OK;
+}
+
+}  // extern "C"

@@ -459,6 +459,42 @@ size_t gdn2_recurrence_marks(int64_t B, int64_t S, const int64_t* cu_seqlens, in
 int gdn2_recurrence_forward(const gdn2_recurrence_args* args, int dtype, void* stream);
 int gdn2_recurrence_backward(const gdn2_recurrence_args* args, int dtype, void* stream);
 
+/*
+ * Gated feed-forward block: y = (act(x Wg^T) * (x Wu^T)) Wd^T, act SiLU or GELU (tanh form); GDN2_BF16 and GDN2_F16, sums in
+ * fp32, what lies between the products (h, a = x Wg^T, u = x Wu^T and their gradients) rounded to `dtype`.
+ *   x [tokens, hidden]  w_gate, w_up [inner, hidden]  w_down [out, inner]  y [tokens, out]
+ *   h, a, u, da, du [tokens, inner] with rows inner_stride elements apart: h is scratch of a forward call; a and u are NULL, or kept
+ *   with h for a backward call; da and du are scratch of the backward call.
+ * gdn2_ffn_backward: dx, (dw_gate, dw_up) and dw_down from dy; a gradient whose pointer is NULL is not computed (dw_gate and dw_up
+ * together; da and du may be NULL if neither they nor dx are wanted). The weights' gradients are contiguous.
+ * Row strides are in ELEMENTS. Inputs, h, a, u, da and du: rows start on 16 bytes (16-byte aligned pointers, strides that are
+ * multiples of 8), else GDN2_ERR_MISALIGNED; gdn2_align_rows copies rows that do not. y, dx and the weights' gradients may have any.
+ * No counterpart in the reference, which has the token mixer alone.
+ */
+enum gdn2_activation { GDN2_ACT_SILU = 0, GDN2_ACT_GELU_TANH = 1 };
+typedef struct gdn2_ffn_args {
+  const void *x, *w_gate, *w_up, *w_down;
+  void *h, *a, *u;
+  void* y;
+  const void* dy;
+  void *da, *du;
+  void *dx, *dw_gate, *dw_up, *dw_down;
+  int64_t tokens, hidden, inner, out;
+  int64_t x_stride, w_gate_stride, w_up_stride, w_down_stride, inner_stride, y_stride, dy_stride, dx_stride;
+  int activation;
+} gdn2_ffn_args;
+
+int gdn2_ffn_forward(const gdn2_ffn_args* args, int dtype, void* stream);
+int gdn2_ffn_backward(const gdn2_ffn_args* args, int dtype, void* stream);
+
+/* Up to 6 matrices of 16-bit elements copied to rows that start on 16 bytes, in one launch; zeros up to the next multiple of 8. */
+typedef struct gdn2_row_copy {
+  const void* src;
+  void* dst;
+  int64_t rows, cols, src_stride, dst_stride;   /* strides in elements; dst 16-byte aligned, dst_stride a multiple of 8 */
+} gdn2_row_copy;
+int gdn2_align_rows(const gdn2_row_copy* copies, int64_t n, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
