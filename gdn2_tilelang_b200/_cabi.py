@@ -67,6 +67,7 @@ SIGNATURES = {
     "gdn2_recurrence_marks": (_sz, [_i64, _i64, ctypes.POINTER(_i64), _i64]),
     "gdn2_recurrence_forward": (_int, [_vp, _int, _vp]),
     "gdn2_recurrence_backward": (_int, [_vp, _int, _vp]),
+    "gdn2_ffn_kept_bytes": (_sz, [_i64, _i64]),
     "gdn2_ffn_forward": (_int, [_vp, _int, _vp]),
     "gdn2_ffn_backward": (_int, [_vp, _int, _vp]),
     "gdn2_align_rows": (_int, [_vp, _i64, _vp]),
@@ -121,7 +122,7 @@ class RecurrenceArgs(ctypes.Structure):
 class FfnArgs(ctypes.Structure):
     """``gdn2_ffn_args`` of include/gdn2_b200.h."""
 
-    _fields_ = ([(n, _vp) for n in ("x", "w_gate", "w_up", "w_down", "h", "a", "u", "y", "dy", "da", "du", "dx", "dw_gate", "dw_up",
+    _fields_ = ([(n, _vp) for n in ("x", "w_gate", "w_up", "w_down", "h", "kept", "y", "dy", "da", "du", "dx", "dw_gate", "dw_up",
                                     "dw_down")]
                 + [(n, _i64) for n in ("tokens", "hidden", "inner", "out", "x_stride", "w_gate_stride", "w_up_stride",
                                        "w_down_stride", "inner_stride", "y_stride", "dy_stride", "dx_stride")]
@@ -268,10 +269,27 @@ class NativeKernels:
         self.lib = load_library()
         self.host = load_host()     # decode, prefill and the layer's decode in one native call, where the case is plain; or None
         self.prefill_path = _PATHS[os.environ.get("GDN2_B200_PREFILL_PATH", "auto")]
-        self.launches = 0   # kernels launched through this object (for the benchmark's accounting)
+        self.launches = 0   # kernels launched through this object and by gradients (for the benchmark's accounting)
         self._side_streams = {}
 
     # -- helpers ---------------------------------------------------------------------------
+    @property
+    def launches(self) -> int:
+        return self._launches + self._gradient_launches()
+
+    @launches.setter
+    def launches(self, n: int):
+        self._launches = n - self._gradient_launches()
+
+    def _gradient_launches(self) -> int:
+        """Kernels that backward passes of the host extension launched."""
+        count = getattr(self.__dict__.get("host"), "gradient_launches", None)
+        return 0 if count is None else count()
+
+    @property
+    def checks_status(self) -> bool:
+        return os.environ.get("GDN2_B200_CHECK_STATUS", "0") not in ("", "0")
+
     @staticmethod
     def _stream(t: torch.Tensor) -> int:
         return torch.cuda.current_stream(t.device).cuda_stream
@@ -665,41 +683,39 @@ class NativeKernels:
         a.tokens, a.hidden = x.shape
         a.out, a.inner = w_down.shape
         a.x_stride, a.w_gate_stride, a.w_up_stride, a.w_down_stride = (_pitch(t) for t in (x, w_gate, w_up, w_down))
-        a.inner_stride = -(-a.inner // 8) * 8
+        a.inner_stride = -(-a.inner // 16) * 16
         a.activation = ACTIVATIONS[activation]
         return a
 
     def ffn_forward(self, x, w_gate, w_up, w_down, activation: str, keep: bool):
-        """``gdn2_ffn_forward`` on rows as ``aligned_rows`` leaves them: ``(y [tokens, out], h, a, u)``; the kept buffers have rows of
-        ``inner`` elements padded to a multiple of 8 (``a``, ``u``: ``None`` without ``keep``)."""
+        """``gdn2_ffn_forward`` on rows as ``aligned_rows`` leaves them: ``(y [tokens, out], kept | None)``; ``kept`` is what
+        ``ffn_backward`` needs of the inner activations."""
         a = self._ffn_args(x, w_gate, w_up, w_down, activation)
-        rows = lambda: torch.empty(a.tokens, a.inner_stride, dtype=x.dtype, device=x.device)     # noqa: E731
         y = torch.empty(a.tokens, a.out, dtype=x.dtype, device=x.device)
-        h, gate, up = rows(), (rows() if keep else None), (rows() if keep else None)
-        a.h, a.a, a.u, a.y, a.y_stride = h.data_ptr(), _ptr(gate), _ptr(up), y.data_ptr(), a.out
+        h = torch.empty(a.tokens, a.inner_stride, dtype=x.dtype, device=x.device)
+        kept = torch.empty(self.lib.gdn2_ffn_kept_bytes(a.tokens, a.inner_stride), dtype=torch.uint8, device=x.device) if keep else None
+        a.h, a.kept, a.y, a.y_stride = h.data_ptr(), _ptr(kept), y.data_ptr(), a.out
         with _on_device(x.device):
             rc = self.lib.gdn2_ffn_forward(ctypes.byref(a), dtype_code(x.dtype), self._stream(x))
         _check(self.lib, rc, "gdn2_ffn_forward")
         self.launches += 2
-        return y, h, gate, up
+        return y, kept
 
-    def ffn_backward(self, x, w_gate, w_up, w_down, h, gate, up, dy, activation: str, want_dx: bool, want_dgate_up: bool,
-                     want_dw_down: bool):
+    def ffn_backward(self, x, w_gate, w_up, w_down, kept, dy, activation: str, want_dx: bool, want_dgate_up: bool, want_dw_down: bool):
         """``gdn2_ffn_backward``: ``(dx, dw_gate, dw_up, dw_down)``, ``None`` where not wanted."""
         a = self._ffn_args(x, w_gate, w_up, w_down, activation)
         new = lambda *shape: torch.empty(*shape, dtype=x.dtype, device=x.device)                 # noqa: E731
-        first = want_dx or want_dgate_up
-        da, du = (new(a.tokens, a.inner_stride), new(a.tokens, a.inner_stride)) if first else (None, None)
+        h, da, du = (new(a.tokens, a.inner_stride) for _ in range(3))
         dx = new(a.tokens, a.hidden) if want_dx else None
         dwg, dwu = (new(a.inner, a.hidden), new(a.inner, a.hidden)) if want_dgate_up else (None, None)
         dwd = new(a.out, a.inner) if want_dw_down else None
-        a.h, a.a, a.u, a.dy, a.dy_stride = h.data_ptr(), gate.data_ptr(), up.data_ptr(), dy.data_ptr(), _pitch(dy)
-        a.da, a.du, a.dx, a.dx_stride = _ptr(da), _ptr(du), _ptr(dx), a.hidden
+        a.h, a.kept, a.dy, a.dy_stride = h.data_ptr(), kept.data_ptr(), dy.data_ptr(), _pitch(dy)
+        a.da, a.du, a.dx, a.dx_stride = da.data_ptr(), du.data_ptr(), _ptr(dx), a.hidden
         a.dw_gate, a.dw_up, a.dw_down = _ptr(dwg), _ptr(dwu), _ptr(dwd)
         with _on_device(x.device):
             rc = self.lib.gdn2_ffn_backward(ctypes.byref(a), dtype_code(x.dtype), self._stream(x))
         _check(self.lib, rc, "gdn2_ffn_backward")
-        self.launches += int(first) + int(want_dx) + int(want_dgate_up) + int(want_dw_down)
+        self.launches += 1 + int(want_dx) + int(want_dgate_up) + int(want_dw_down)
         return dx, dwg, dwu, dwd
 
     # -- diagnostics -------------------------------------------------------------------------
@@ -813,7 +829,7 @@ class NativeKernels:
         """With ``GDN2_B200_CHECK_STATUS=1`` every public call ends with a synchronising status check, so a
         kernel that gave up on a bounded wait raises at the call that launched it (debugging aid; off by default
         because it serialises the host with the device)."""
-        if os.environ.get("GDN2_B200_CHECK_STATUS", "0") not in ("", "0"):
+        if self.checks_status:
             if torch.cuda.is_current_stream_capturing():
                 return                   # a captured stream cannot be synchronised; the replaying caller checks
             self.check_device_status(device)

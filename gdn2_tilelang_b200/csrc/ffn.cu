@@ -2,7 +2,7 @@
 //
 //   forward   a = x Wg^T, u = x Wu^T, h = act(a) u     one kernel: both projections, the activation and the product
 //             y = h Wd^T
-//   backward  dh = dy Wd, da = dh u act'(a), du = dh act(a)      one kernel
+//   backward  dh = dy Wd, da = dh u act'(a), du = dh act(a), h again      one kernel
 //             dx = da Wg + du Wu                                 one kernel (the two products are one long reduction)
 //             dWg = da^T x, dWu = du^T x;  dWd = dy^T h          a kernel each
 //
@@ -15,16 +15,18 @@
 //
 // In the forward product block 0 of a pair brings rows of Wg as its half of B and block 1 the same rows of Wu: columns c and 128 + c of
 // the tile are then the gate and the up projection of one inner channel, in the same lane of tensor memory, and the epilogue
-// needs nothing from another thread. h, and for a training step a and u, are rounded to 16 bits there: they are what the next
-// product reads, and a tensor core reads 16 bits. The sums before and after are fp32.
+// needs nothing from another thread. h is rounded to 16 bits there: it is what the next product reads, and a tensor core reads
+// 16 bits. The same holds for da and du. Everything else stays fp32 up to the results, with one exception: what a training step
+// keeps of a and u are the upper 24 bits of their fp32 sums, 16 in one plane and 8 in another. In 16 bits their rounding weighs as
+// much as that of da or of the result (dx off by 3.1e-3 of its 2-norm in bf16, with 24 bits by 2.4e-3); keeping them so and forming h a second
+// time in the backward pass takes the 6 bytes an inner channel that a, u and h take in 16 bits.
 //
 // Few tokens (skinny_kernel): the work is reading the weights once. They take the 128-row side of the product, the tokens
 // the narrow one, and the reduction of a tile is cut over the blocks of a cluster so that every SM reads; the blocks' partial
 // sums meet in distributed shared memory, added in the order of the blocks.
-#include <cuda.h>
-
 #include "common.cuh"
 #include "tc_utils.cuh"
+#include "tensor_map.cuh"
 
 namespace gdn2 {
 
@@ -41,25 +43,40 @@ constexpr uint32_t kWaitCode = 1u << 28;
 
 enum Kind { kPlain = 0, kGated = 1, kGatedBackward = 2 };
 
-// Stages that fit beside a kind's staging buffers: one chunk a warp, two in and out for the backward epilogue.
-template <int K> __host__ __device__ constexpr int stages() { return K == kGatedBackward ? 5 : 6; }
-template <int K> __host__ __device__ constexpr int staging_bytes() { return kEpiWarps * kChunkBytes * (K == kGatedBackward ? 2 : 1); }
+// Stages that fit beside a kind's staging buffers: one chunk a warp, three in and out for the backward epilogue.
+template <int K> __host__ __device__ constexpr int stages() { return K == kGatedBackward ? 4 : 6; }
+template <int K> __host__ __device__ constexpr int staging_bytes() { return kEpiWarps * kChunkBytes * (K == kGatedBackward ? 3 : 1); }
 template <int K> constexpr size_t smem_bytes() { return (size_t)stages<K>() * kStageBytes + staging_bytes<K>() + 1024; }
 
 struct __align__(64) Maps {
   CUtensorMap a[2], b[2];       // kPlain: operands of the one or two runs of reduction steps; kGated: b = Wg, Wu
-  CUtensorMap out[3];           // kPlain: result (of the upper and of the lower tiles); kGated: h, a, u; kGatedBackward: da, du
-  CUtensorMap in[2];            // kGatedBackward: a, u
+  CUtensorMap out[3];           // kPlain: result (of the upper and of the lower tiles); kGated: h; kGatedBackward: da, du, h
+  CUtensorMap kept[4];          // the planes of a and u: upper 16 bits of a, of u, lower 8 of a, of u
 };
 struct Problem {
   int steps[2];                 // stages of the two runs (steps[1] = 0: one run)
   int tiles_m, tiles_n;
   int split_m;                  // > 0: tiles from this one on take a[1] and out[1], their rows counted from there (dWg, dWu)
   int M, N;                     // rows and columns of the result (of one part)
-  int save, gelu;
+  int save, gelu;               // kGated: a and u are kept; kGatedBackward: h is wanted
   void* plain_out[2];           // results whose rows do not start on 16 bytes are stored by threads
   int64_t out_stride;
 };
+
+// The planes of a and u inside a kept buffer of 6 tokens * stride bytes
+struct Planes {
+  uint16_t* upper[2];
+  uint8_t* lower[2];
+};
+__host__ __device__ inline Planes planes(void* kept, int64_t tokens, int64_t stride) {
+  const int64_t n = tokens * stride;
+  Planes p;
+  p.upper[0] = static_cast<uint16_t*>(kept);
+  p.upper[1] = p.upper[0] + n;
+  p.lower[0] = reinterpret_cast<uint8_t*>(p.upper[1] + n);
+  p.lower[1] = p.lower[0] + n;
+  return p;
+}
 
 // ---------------------------------------------------------------- instructions
 
@@ -169,6 +186,36 @@ template <typename T> __device__ __forceinline__ void get_row(const char* chunk,
     const T* e = reinterpret_cast<const T*>(&r);
 #pragma unroll
     for (int i = 0; i < 8; ++i) x[8 * j + i] = to_f32<T>(e[i]);
+  }
+}
+// The upper 24 bits of two or four numbers, rounded (ties away from zero; a number within 2^-17 of the largest becomes infinite).
+// A NaN keeps its upper 16 bits, whose quiet bit is set.
+__device__ __forceinline__ uint32_t round24(float x) {
+  const uint32_t b = __float_as_uint(x);
+  return (b & 0x7fffffffu) > 0x7f800000u ? b : b + 0x80u;
+}
+__device__ __forceinline__ uint32_t upper16(uint32_t b0, uint32_t b1) { return __byte_perm(b0, b1, 0x7632); }
+__device__ __forceinline__ uint32_t lower8(uint32_t b0, uint32_t b1, uint32_t b2, uint32_t b3) {
+  return __byte_perm(__byte_perm(b0, b1, 0x0051), __byte_perm(b2, b3, 0x0051), 0x5410);
+}
+// 32 columns from `first` (0 or 32) of this lane's row of a plane's chunk, from rounded numbers and back. The lower plane's rows
+// are 64 bytes, swizzled in 64-byte rows as TMA does it.
+__device__ __forceinline__ void put_upper(char* chunk, int lane, int first, const uint32_t (&b)[32]) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+    *reinterpret_cast<uint4*>(chunk + lane * 128 + (((first / 8 + j) ^ (lane & 7)) * 16)) =
+        make_uint4(upper16(b[8 * j], b[8 * j + 1]), upper16(b[8 * j + 2], b[8 * j + 3]), upper16(b[8 * j + 4], b[8 * j + 5]),
+                   upper16(b[8 * j + 6], b[8 * j + 7]));
+}
+__device__ __forceinline__ uint32_t lower_at(int lane, int j) { return lane * 64 + ((j ^ ((lane >> 1) & 3)) * 16); }
+__device__ __forceinline__ void get_kept(const char* upper, const uint4 (&lower)[4], int lane, int first, float (&x)[32]) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const uint4 r = *reinterpret_cast<const uint4*>(upper + lane * 128 + (((first / 8 + j) ^ (lane & 7)) * 16));
+    const uint32_t h[4] = {r.x, r.y, r.z, r.w}, *l = reinterpret_cast<const uint32_t*>(&lower[first / 16 + j / 2]) + 2 * (j & 1);
+#pragma unroll
+    for (int i = 0; i < 8; ++i)       // two bytes of the upper plane, one of the lower
+      x[8 * j + i] = __uint_as_float(__byte_perm(h[i / 2], l[i / 4], (i & 1 ? 0x3200 : 0x1000) | (4 + (i & 3)) << 4) & 0xffffff00u);
   }
 }
 // A warp's chunk to rows row.., columns col.. of the result; what lies outside is dropped.
@@ -335,9 +382,12 @@ product_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Proble
       tile_at(p, i, m, n);
       if (lane == 0) {
         const int row = m * kTile + rank * kBlockRows + quad * 32, col = n * kTile + half * 128 + c * kChunk16;
-        tc::mbar_expect_tx(&sh.loaded[ew], 2 * kChunkBytes);
-        tma_load(tc::smem_u32(chunk), &maps.in[0], col, row, tc::smem_u32(&sh.loaded[ew]));
-        tma_load(tc::smem_u32(chunk + kChunkBytes), &maps.in[1], col, row, tc::smem_u32(&sh.loaded[ew]));
+        const uint32_t bar = tc::smem_u32(&sh.loaded[ew]), at = tc::smem_u32(chunk);
+        tc::mbar_expect_tx(&sh.loaded[ew], 3 * kChunkBytes);
+        tma_load(at, &maps.kept[0], col, row, bar);
+        tma_load(at + kChunkBytes, &maps.kept[1], col, row, bar);
+        tma_load(at + 2 * kChunkBytes, &maps.kept[2], col, row, bar);
+        tma_load(at + 2 * kChunkBytes + kChunkBytes / 2, &maps.kept[3], col, row, bar);
       }
     };
     if constexpr (K == kGatedBackward) load_chunk(pair, 0);
@@ -368,41 +418,45 @@ product_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Proble
         }
       } else if constexpr (K == kGated) {
         const int col = n * kBlockRows + half * kChunk16;
-        uint32_t a16[32], u16[32];                    // a and u as they are kept, in pairs
+        uint32_t alow[16], ulow[16];                  // the lower planes
 #pragma unroll
-        for (int q = 0; q < 2; ++q) {
-          float a[32], u[32];
-          tc::tmem_ld32(acc + half * kChunk16 + 32 * q, a);
-          tc::tmem_ld32(acc + kBlockRows + half * kChunk16 + 32 * q, u);
-          tc::tmem_ld_wait();
-          if (p.save) {
+        for (int part = 0; part < 3; ++part) {        // h, then the upper planes; the tile is read again for each rather than held
+          if (part > 0 && !p.save) break;
+          chunk_free(lane);
 #pragma unroll
-            for (int j = 0; j < 16; ++j) {
-              a16[16 * q + j] = pack2<T>(a[2 * j], a[2 * j + 1]);
-              u16[16 * q + j] = pack2<T>(u[2 * j], u[2 * j + 1]);
+          for (int q = 0; q < 2; ++q) {
+            float a[32], u[32];
+            if (part != 2) tc::tmem_ld32(acc + half * kChunk16 + 32 * q, a);
+            if (part != 1) tc::tmem_ld32(acc + kBlockRows + half * kChunk16 + 32 * q, u);
+            tc::tmem_ld_wait();
+            if (part == 0) {
+#pragma unroll
+              for (int j = 0; j < 32; ++j) {
+                float none;
+                a[j] = activate<false>(a[j], p.gelu, none) * u[j];
+              }
+              put_row<T>(chunk, lane, 32 * q, a);
+            } else {
+              uint32_t b[32], (&low)[16] = part == 1 ? alow : ulow;
+#pragma unroll
+              for (int j = 0; j < 32; ++j) b[j] = round24(part == 1 ? a[j] : u[j]);
+              put_upper(chunk, lane, 32 * q, b);
+#pragma unroll
+              for (int j = 0; j < 8; ++j) low[8 * q + j] = lower8(b[4 * j], b[4 * j + 1], b[4 * j + 2], b[4 * j + 3]);
             }
           }
-#pragma unroll
-          for (int j = 0; j < 32; ++j) {
-            float none;
-            a[j] = activate<false>(a[j], p.gelu, none) * u[j];
-          }
-          if (q == 0) chunk_free(lane);
-          put_row<T>(chunk, lane, 32 * q, a);
+          store_chunk<T>(chunk, part == 0 ? &maps.out[0] : &maps.kept[part - 1], nullptr, 0, row, col, p.M, p.N, lane);
         }
-        store_chunk<T>(chunk, &maps.out[0], nullptr, 0, row, col, p.M, p.N, lane);
         if (p.save) {
+          chunk_free(lane);
 #pragma unroll
-          for (int part = 0; part < 2; ++part) {
-            chunk_free(lane);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-              const uint32_t* w = part ? u16 : a16;
-              *reinterpret_cast<uint4*>(chunk + lane * 128 + ((j ^ (lane & 7)) * 16)) =
-                  make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
-            }
-            store_chunk<T>(chunk, &maps.out[1 + part], nullptr, 0, row, col, p.M, p.N, lane);
+          for (int j = 0; j < 4; ++j) {
+            *reinterpret_cast<uint4*>(chunk + lower_at(lane, j)) = make_uint4(alow[4 * j], alow[4 * j + 1], alow[4 * j + 2], alow[4 * j + 3]);
+            *reinterpret_cast<uint4*>(chunk + kChunkBytes / 2 + lower_at(lane, j)) =
+                make_uint4(ulow[4 * j], ulow[4 * j + 1], ulow[4 * j + 2], ulow[4 * j + 3]);
           }
+          store_chunk<T>(chunk, &maps.kept[2], nullptr, 0, row, col, p.M, p.N, lane);
+          store_chunk<T>(chunk + kChunkBytes / 2, &maps.kept[3], nullptr, 0, row, col, p.M, p.N, lane);
         }
       } else {
         bool ok = true;
@@ -412,25 +466,38 @@ product_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Proble
           ok = tc::mbar_wait_warp(&sh.loaded[ew], loads & 1, &sh.abort, status, kWaitCode);
           if (!ok) break;
           ++loads;
+          uint4 alow[4], ulow[4];
+          char* third = chunk + 2 * kChunkBytes;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            alow[j] = *reinterpret_cast<const uint4*>(third + lower_at(lane, j));
+            ulow[j] = *reinterpret_cast<const uint4*>(third + kChunkBytes / 2 + lower_at(lane, j));
+          }
+          __syncwarp();                               // h takes the lower planes' place
 #pragma unroll
           for (int q = 0; q < 2; ++q) {
             float d[32], a[32], u[32];
             tc::tmem_ld32(acc + at + 32 * q, d);
-            get_row<T>(chunk, lane, 32 * q, a);
-            get_row<T>(chunk + kChunkBytes, lane, 32 * q, u);
+            get_kept(chunk, alow, lane, 32 * q, a);
+            get_kept(chunk + kChunkBytes, ulow, lane, 32 * q, u);
             tc::tmem_ld_wait();
+            float h[32];
 #pragma unroll
             for (int j = 0; j < 32; ++j) {
               float slope;
               const float act = activate<true>(a[j], p.gelu, slope);
+              h[j] = act * u[j];
               a[j] = d[j] * u[j] * slope;
               u[j] = d[j] * act;
             }
             put_row<T>(chunk, lane, 32 * q, a);
             put_row<T>(chunk + kChunkBytes, lane, 32 * q, u);
+            put_row<T>(third, lane, 32 * q, h);
           }
-          store_chunk<T>(chunk, &maps.out[0], nullptr, 0, row, n * kTile + at, p.M, p.N, lane);
-          store_chunk<T>(chunk + kChunkBytes, &maps.out[1], nullptr, 0, row, n * kTile + at, p.M, p.N, lane);
+          const int col = n * kTile + at;
+          store_chunk<T>(chunk, &maps.out[0], nullptr, 0, row, col, p.M, p.N, lane);
+          store_chunk<T>(chunk + kChunkBytes, &maps.out[1], nullptr, 0, row, col, p.M, p.N, lane);
+          if (p.save) store_chunk<T>(third, &maps.out[2], nullptr, 0, row, col, p.M, p.N, lane);
           tc::fence_async_smem();                     // a chunk outside the result was not stored: order its rewriting all the same
           chunk_free(lane);
           if (c == 0) load_chunk(i, 1); else load_chunk(i + pairs, 0);
@@ -468,8 +535,9 @@ struct Skinny {
   int tokens, width;                             // width: tokens rounded up to 16
   int rows;                                      // weight rows: inner channels, or outputs
   int gelu;
-  void *out, *a, *u;                             // a, u: kept for a backward pass, or null
-  int64_t out_stride, au_stride;
+  void* out;
+  void* kept;                                    // what a backward pass needs of a and u, or null
+  int64_t out_stride, kept_stride;
 };
 
 template <typename T, bool Gated>
@@ -578,9 +646,15 @@ __global__ void __launch_bounds__(kSkinnyThreads, 1) skinny_kernel(const __grid_
         if constexpr (Gated) {
           float none;
           *out = from_f32<T>(activate<false>(v[0], p.gelu, none) * v[1]);
-          if (p.a) {
-            static_cast<T*>(p.a)[(int64_t)n * p.au_stride + row] = from_f32<T>(v[0]);
-            static_cast<T*>(p.u)[(int64_t)n * p.au_stride + row] = from_f32<T>(v[1]);
+          if (p.kept) {
+            const Planes k = planes(p.kept, p.tokens, p.kept_stride);
+            const int64_t e = (int64_t)n * p.kept_stride + row;
+#pragma unroll
+            for (int g = 0; g < 2; ++g) {
+              const uint32_t b = round24(v[g]);
+              k.upper[g][e] = (uint16_t)(b >> 16);
+              k.lower[g][e] = (uint8_t)(b >> 8);
+            }
           }
         } else {
           *out = from_f32<T>(v[0]);
@@ -618,43 +692,31 @@ __global__ void __launch_bounds__(256) align_rows_kernel(const __grid_constant__
 
 // ---------------------------------------------------------------- host side
 
-using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
-                                 const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
-                                 CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-EncodeTiled encode_tiled() {
-  static const EncodeTiled fn = [] {
-    void* p = nullptr;
-    cudaDriverEntryPointQueryResult q;
-    if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &p, 12000, cudaEnableDefault, &q) != cudaSuccess ||
-        q != cudaDriverEntryPointSuccess)
-      p = nullptr;
-    return reinterpret_cast<EncodeTiled>(p);
-  }();
-  return fn;
-}
-
 // a [rows, cols] matrix of 16-bit elements with rows `stride` elements apart, in boxes of box_rows x 64
 struct Matrix {
   const void* p;
   int64_t rows, cols, stride;
 };
-bool make_map(CUtensorMap* map, const Matrix& m, int box_rows, int dtype) {
+bool make_map(CUtensorMap* map, const Matrix& m, int box_rows, CUtensorMapDataType type, int size) {
   const EncodeTiled fn = encode_tiled();
   if (!fn) return false;
-  const cuuint64_t dims[2] = {(cuuint64_t)m.cols, (cuuint64_t)m.rows}, strides[1] = {(cuuint64_t)m.stride * 2};
+  const cuuint64_t dims[2] = {(cuuint64_t)m.cols, (cuuint64_t)m.rows}, strides[1] = {(cuuint64_t)m.stride * size};
   const cuuint32_t box[2] = {64, (cuuint32_t)box_rows}, unit[2] = {1, 1};
-  return fn(map, dtype == GDN2_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, const_cast<void*>(m.p), dims,
-            strides, box, unit, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+  return fn(map, type, 2, const_cast<void*>(m.p), dims, strides, box, unit, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            size == 2 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
-
-// Encoding a map is a driver call that needs the device's context to be the thread's own, which a thread that has made no runtime
-// call yet (an autograd engine's) lacks.
-int own_context() {
-  int dev = 0;
-  GDN2_CUDA_TRY(cudaGetDevice(&dev));
-  GDN2_CUDA_TRY(cudaSetDevice(dev));
-  return GDN2_OK;
+bool make_map(CUtensorMap* map, const Matrix& m, int box_rows, int dtype) {
+  return make_map(map, m, box_rows, dtype == GDN2_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2);
+}
+// the planes of a kept buffer
+bool make_kept_maps(CUtensorMap (&maps)[4], void* kept, const Matrix& h) {
+  const Planes k = planes(kept, h.rows, h.stride);
+  for (int g = 0; g < 2; ++g)
+    if (!make_map(&maps[g], Matrix{k.upper[g], h.rows, h.cols, h.stride}, 32, CU_TENSOR_MAP_DATA_TYPE_UINT16, 2) ||
+        !make_map(&maps[2 + g], Matrix{k.lower[g], h.rows, h.cols, h.stride}, 32, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1))
+      return false;
+  return true;
 }
 
 bool aligned_rows(const Matrix& m) { return (reinterpret_cast<uintptr_t>(m.p) & 15u) == 0 && m.stride % 8 == 0; }
@@ -678,42 +740,39 @@ int launch_product(const Maps& maps, const Problem& p, cudaStream_t st) {
     if (!make_map(&(m), matrix, box, dtype)) return GDN2_ERR_UNSUPPORTED; \
   } while (0)
 
-// h (and a, u) = the gated product of x and Wg, Wu
+// h (and what is kept of a, u) = the gated product of x and Wg, Wu
 template <typename T>
-int gated_forward(const Matrix& x, const Matrix& wg, const Matrix& wu, const Matrix& h, const Matrix* a, const Matrix* u, int gelu, int dtype,
-                  cudaStream_t st) {
+int gated_forward(const Matrix& x, const Matrix& wg, const Matrix& wu, const Matrix& h, void* kept, int gelu, int dtype, cudaStream_t st) {
   Maps maps{};
   Problem p{};
   GDN2_MAP(maps.a[0], x, kBlockRows);
   GDN2_MAP(maps.b[0], wg, kBlockRows);
   GDN2_MAP(maps.b[1], wu, kBlockRows);
   GDN2_MAP(maps.out[0], h, 32);
-  if (a) {
-    GDN2_MAP(maps.out[1], *a, 32);
-    GDN2_MAP(maps.out[2], *u, 32);
-  }
+  if (kept && !make_kept_maps(maps.kept, kept, h)) return GDN2_ERR_UNSUPPORTED;
   p.steps[0] = steps_of(x.cols);
   p.tiles_m = tiles_of(x.rows, kTile);
   p.tiles_n = tiles_of(wg.rows, kBlockRows);
   p.M = (int)x.rows;
   p.N = (int)wg.rows;
-  p.save = a != nullptr;
+  p.save = kept != nullptr;
   p.gelu = gelu;
   return launch_product<T, kGated, false, false>(maps, p, st);
 }
 
-// da, du from dy, Wd and the kept a, u
+// da, du (and h) from dy, Wd and what was kept of a, u
 template <typename T>
-int gated_backward(const Matrix& dy, const Matrix& wd, const Matrix& a, const Matrix& u, const Matrix& da, const Matrix& du, int gelu,
+int gated_backward(const Matrix& dy, const Matrix& wd, void* kept, const Matrix& da, const Matrix& du, const Matrix& h, bool want_h, int gelu,
                    int dtype, cudaStream_t st) {
   Maps maps{};
   Problem p{};
   GDN2_MAP(maps.a[0], dy, kBlockRows);
   GDN2_MAP(maps.b[0], wd, kStep);
-  GDN2_MAP(maps.in[0], a, 32);
-  GDN2_MAP(maps.in[1], u, 32);
+  if (!make_kept_maps(maps.kept, kept, h)) return GDN2_ERR_UNSUPPORTED;
   GDN2_MAP(maps.out[0], da, 32);
   GDN2_MAP(maps.out[1], du, 32);
+  GDN2_MAP(maps.out[2], h, 32);
+  p.save = want_h;
   p.steps[0] = steps_of(dy.cols);
   p.tiles_m = tiles_of(dy.rows, kTile);
   p.tiles_n = tiles_of(wd.cols, kTile);
@@ -769,8 +828,8 @@ int two_weight_gradients(const Matrix& a0, const Matrix& a1, const Matrix& b, co
 }
 
 template <typename T, bool Gated>
-int launch_skinny(const Matrix& x, const Matrix& w0, const Matrix* w1, const Matrix& out, void* a, void* u, int64_t au_stride, int gelu,
-                  int dtype, cudaStream_t st) {
+int launch_skinny(const Matrix& x, const Matrix& w0, const Matrix* w1, const Matrix& out, void* kept, int64_t kept_stride, int gelu, int dtype,
+                  cudaStream_t st) {
   SkinnyMaps maps{};
   Skinny p{};
   p.tokens = (int)x.rows;
@@ -783,7 +842,8 @@ int launch_skinny(const Matrix& x, const Matrix& w0, const Matrix* w1, const Mat
   p.gelu = gelu;
   p.out = const_cast<void*>(out.p);
   p.out_stride = out.stride;
-  p.a = a; p.u = u; p.au_stride = au_stride;
+  p.kept = kept;
+  p.kept_stride = kept_stride;
   p.stage_bytes = (Gated ? 2 : 1) * kOperandBytes + p.width * kStep * 2;
   p.stages = (220 * 1024) / p.stage_bytes;
   if (p.stages > 8) p.stages = 8;
@@ -819,15 +879,15 @@ int launch_skinny(const Matrix& x, const Matrix& w0, const Matrix* w1, const Mat
 template <typename T> int forward(const gdn2_ffn_args& f, int dtype, cudaStream_t st) {
   const Matrix x{f.x, f.tokens, f.hidden, f.x_stride}, wg{f.w_gate, f.inner, f.hidden, f.w_gate_stride},
       wu{f.w_up, f.inner, f.hidden, f.w_up_stride}, wd{f.w_down, f.out, f.inner, f.w_down_stride}, h{f.h, f.tokens, f.inner, f.inner_stride},
-      y{f.y, f.tokens, f.out, f.y_stride}, a{f.a, f.tokens, f.inner, f.inner_stride}, u{f.u, f.tokens, f.inner, f.inner_stride};
+      y{f.y, f.tokens, f.out, f.y_stride};
   const int gelu = f.activation == GDN2_ACT_GELU_TANH;
   int rc;
   if (f.tokens <= kSkinnyTokens) {
-    rc = launch_skinny<T, true>(x, wg, &wu, h, f.a, f.u, f.inner_stride, gelu, dtype, st);
+    rc = launch_skinny<T, true>(x, wg, &wu, h, f.kept, f.inner_stride, gelu, dtype, st);
     if (rc != GDN2_OK) return rc;
-    return launch_skinny<T, false>(h, wd, nullptr, y, nullptr, nullptr, 0, 0, dtype, st);
+    return launch_skinny<T, false>(h, wd, nullptr, y, nullptr, 0, 0, dtype, st);
   }
-  rc = gated_forward<T>(x, wg, wu, h, f.a ? &a : nullptr, &u, gelu, dtype, st);
+  rc = gated_forward<T>(x, wg, wu, h, f.kept, gelu, dtype, st);
   if (rc != GDN2_OK) return rc;
   return product<T, false, false>(&h, &wd, 1, y, dtype, st);
 }
@@ -835,11 +895,10 @@ template <typename T> int forward(const gdn2_ffn_args& f, int dtype, cudaStream_
 template <typename T> int backward(const gdn2_ffn_args& f, int dtype, cudaStream_t st) {
   const Matrix x{f.x, f.tokens, f.hidden, f.x_stride}, wg{f.w_gate, f.inner, f.hidden, f.w_gate_stride},
       wu{f.w_up, f.inner, f.hidden, f.w_up_stride}, wd{f.w_down, f.out, f.inner, f.w_down_stride}, h{f.h, f.tokens, f.inner, f.inner_stride},
-      a{f.a, f.tokens, f.inner, f.inner_stride}, u{f.u, f.tokens, f.inner, f.inner_stride}, dy{f.dy, f.tokens, f.out, f.dy_stride},
+      dy{f.dy, f.tokens, f.out, f.dy_stride},
       da{f.da, f.tokens, f.inner, f.inner_stride}, du{f.du, f.tokens, f.inner, f.inner_stride}, dx{f.dx, f.tokens, f.hidden, f.dx_stride},
       dwg{f.dw_gate, f.inner, f.hidden, f.hidden}, dwu{f.dw_up, f.inner, f.hidden, f.hidden}, dwd{f.dw_down, f.out, f.inner, f.inner};
-  int rc = GDN2_OK;
-  if (f.dx || f.dw_gate) rc = gated_backward<T>(dy, wd, a, u, da, du, f.activation == GDN2_ACT_GELU_TANH, dtype, st);
+  int rc = gated_backward<T>(dy, wd, f.kept, da, du, h, f.dw_down != nullptr, f.activation == GDN2_ACT_GELU_TANH, dtype, st);
   if (rc == GDN2_OK && f.dx) {
     const Matrix lhs[2] = {da, du}, rhs[2] = {wg, wu};
     rc = product<T, false, true>(lhs, rhs, 2, dx, dtype, st);
@@ -862,18 +921,18 @@ int check(const gdn2_ffn_args& f, int dtype, bool back) {
     return GDN2_ERR_BAD_SHAPE;
   if (!f.x || !f.w_gate || !f.w_up || !f.w_down || !f.h) return GDN2_ERR_NULL_POINTER;
   if (back) {
-    if (!f.dy || !f.a || !f.u) return GDN2_ERR_NULL_POINTER;
-    if ((f.dx || f.dw_gate) && (!f.da || !f.du)) return GDN2_ERR_NULL_POINTER;
+    if (!f.dy || !f.kept || !f.da || !f.du) return GDN2_ERR_NULL_POINTER;
     if ((f.dw_gate == nullptr) != (f.dw_up == nullptr)) return GDN2_ERR_NULL_POINTER;
   } else {
-    if (!f.y || (f.a == nullptr) != (f.u == nullptr)) return GDN2_ERR_NULL_POINTER;
+    if (!f.y) return GDN2_ERR_NULL_POINTER;
   }
   if (f.x_stride < f.hidden || f.w_gate_stride < f.hidden || f.w_up_stride < f.hidden || f.w_down_stride < f.inner ||
       f.inner_stride < f.inner || (back ? f.dy_stride < f.out || (f.dx && f.dx_stride < f.hidden) : f.y_stride < f.out))
     return GDN2_ERR_BAD_SHAPE;
   for (int64_t s : {f.x_stride, f.w_gate_stride, f.w_up_stride, f.w_down_stride, f.inner_stride, back ? f.dy_stride : (int64_t)0})
     if (s % 8 || s > (1LL << 34)) return GDN2_ERR_MISALIGNED;
-  for (const void* q : {f.x, f.w_gate, f.w_up, f.w_down, (const void*)f.h, (const void*)f.a, (const void*)f.u, back ? f.dy : nullptr,
+  if (f.inner_stride % 16) return GDN2_ERR_MISALIGNED;        // rows of the byte planes start on 16 bytes, too
+  for (const void* q : {f.x, f.w_gate, f.w_up, f.w_down, (const void*)f.h, (const void*)f.kept, back ? f.dy : nullptr,
                         back ? (const void*)f.da : nullptr, back ? (const void*)f.du : nullptr})
     if (reinterpret_cast<uintptr_t>(q) & 15u) return GDN2_ERR_MISALIGNED;
   return GDN2_OK;
@@ -883,6 +942,10 @@ int check(const gdn2_ffn_args& f, int dtype, bool back) {
 }  // namespace gdn2
 
 extern "C" {
+
+size_t gdn2_ffn_kept_bytes(int64_t tokens, int64_t inner_stride) {
+  return tokens > 0 && inner_stride > 0 ? (size_t)tokens * (size_t)inner_stride * 6 : 0;
+}
 
 int gdn2_ffn_forward(const gdn2_ffn_args* args, int dtype, void* stream) {
   if (!args) return GDN2_ERR_NULL_POINTER;

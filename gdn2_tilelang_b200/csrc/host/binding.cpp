@@ -5,12 +5,17 @@
 // Every function takes the plain case only -- dense, aligned CUDA tensors of the expected shapes and types on the
 // current device -- and returns None for anything else, so that the general path in Python handles it or raises the
 // error that belongs to it. Nothing is kept between calls.
+#include <atomic>
+
 #include <ATen/ATen.h>
 #include <ATen/autocast_mode.h>
 #include <ATen/core/grad_mode.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/cuda/CUDAFunctions.h>
+#include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/utils/pybind.h>
 
 #include "../../../include/gdn2_b200.h"
@@ -281,6 +286,243 @@ std::optional<std::tuple<Tensor, Tensor, Tensor, int64_t>> layer_prefill(Tensor 
   return std::make_tuple(std::get<0>(*res), fin, std::get<1>(*res), std::get<2>(*res) + launched);
 }
 
+// ---------------------------------------------------------------- the differentiable operators
+
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+std::atomic<int64_t> g_gradient_launches{0};      // kernels launched by backward passes, which return to autograd and not to the caller
+
+void check(int rc, const char* what) {
+  if (rc != GDN2_OK)
+    throw std::runtime_error(std::string(what) + ": " + gdn2_status_string(rc) +
+                             (rc == GDN2_ERR_CUDA ? " (cudaError " + std::to_string(gdn2_last_cuda_error()) + ")" : "") + " [status " +
+                             std::to_string(rc) + "]");
+}
+bool wants_grad(std::initializer_list<const Tensor*> ts) {
+  if (!at::GradMode::is_enabled()) return false;
+  for (const Tensor* t : ts)
+    if (t->defined() && t->requires_grad()) return true;
+  return false;
+}
+// Gradients that were asked for with create_graph: there is no second derivative, and using one says so.
+variable_list once(variable_list grads, const char* what) {
+  if (!at::GradMode::is_enabled()) return grads;
+  variable_list live;
+  for (const Tensor& t : grads)
+    if (t.defined()) live.push_back(t.set_requires_grad(true));      // new tensors of the pass's own, so that the error is attached
+  auto error = std::make_shared<torch::autograd::DelayedError>(std::string(what) + " is differentiable once", (int64_t)live.size());
+  live = (*error)(std::move(live));
+  size_t i = 0;
+  for (Tensor& t : grads)
+    if (t.defined()) t = live[i++];
+  return grads;
+}
+void* stream_on(const Tensor& t) { return c10::cuda::getCurrentCUDAStream(t.get_device()).stream(); }
+template <typename T> T* ptr(const Tensor& t) { return t.defined() ? static_cast<T*>(t.data_ptr()) : nullptr; }
+
+// [B, S, ...] as rows [B, S, D] whose channels lie side by side, or an undefined tensor
+Tensor as_rows(const Tensor& t) {
+  if (t.dim() < 3) return Tensor();
+  Tensor r = t.dim() == 3 ? t : t.is_contiguous() ? t.view({t.size(0), t.size(1), -1}) : Tensor();
+  if (r.defined() && r.size(2) > 1 && r.stride(2) != 1) return Tensor();
+  return r;
+}
+void set_rows(const Tensor& t, const void** p, int64_t* batch, int64_t* token) {
+  *p = t.data_ptr();
+  *batch = t.size(0) > 1 ? t.stride(0) : 0;
+  *token = t.size(1) > 1 ? t.stride(1) : 0;
+}
+gdn2_recurrence_args recurrence_args(const Tensor& v, const Tensor& g, const Tensor& w, const std::vector<int64_t>& offsets) {
+  gdn2_recurrence_args a{};
+  const void* pg = nullptr;
+  set_rows(v, &a.v, &a.v_batch_stride, &a.v_token_stride);
+  set_rows(g, &pg, &a.g_batch_stride, &a.g_token_stride);
+  a.g = static_cast<const float*>(pg);
+  if (w.defined()) set_rows(w, &a.w, &a.w_batch_stride, &a.w_token_stride);
+  a.B = v.size(0); a.S = v.size(1); a.D = v.size(2);
+  a.sequences = offsets.empty() ? a.B : (int64_t)offsets.size() - 1;
+  a.cu_seqlens = offsets.empty() ? nullptr : offsets.data();
+  return a;
+}
+int64_t recurrence_launches(const gdn2_recurrence_args& a) { return a.cu_seqlens ? (a.sequences + 127) / 128 : 1; }
+
+struct Recurrence : torch::autograd::Function<Recurrence> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& v, const Tensor& g, const std::optional<Tensor>& gate,
+                               const std::optional<Tensor>& initial, const std::vector<int64_t>& offsets) {
+    const Tensor w = gate.value_or(Tensor()), state = initial.value_or(Tensor());
+    gdn2_recurrence_args a = recurrence_args(v, g, w, offsets);
+    const auto opt = v.options().requires_grad(false);
+    Tensor o = at::empty(v.sizes(), opt), final = at::empty({a.sequences, a.D}, opt.dtype(at::kFloat));
+    Tensor marks = at::empty({(int64_t)gdn2_recurrence_marks(a.B, a.S, a.cu_seqlens, a.sequences), a.D}, opt.dtype(at::kFloat));
+    a.state = ptr<float>(state); a.o = o.data_ptr(); a.final_state = ptr<float>(final); a.marks = ptr<float>(marks);
+    check(gdn2_recurrence_forward(&a, dtype_code(v.scalar_type()), stream_on(v)), "gdn2_recurrence_forward");
+    ctx->save_for_backward({v, g, w, marks});
+    ctx->saved_data["offsets"] = offsets;
+    ctx->saved_data["state"] = state.defined();
+    ctx->set_materialize_grads(false);
+    return {o, final};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    if (!grads[0].defined() && !grads[1].defined()) return variable_list(5);
+    const auto saved = ctx->get_saved_variables();
+    variable_list out(5);
+    {
+      at::NoGradGuard no_grad;
+      const Tensor &v = saved[0], &g = saved[1], &w = saved[2], &marks = saved[3];
+      const c10::cuda::CUDAGuard device(v.device());
+      const std::vector<int64_t> offsets = ctx->saved_data["offsets"].toIntVector();
+      gdn2_recurrence_args a = recurrence_args(v, g, w, offsets);
+      const auto opt = v.options().requires_grad(false);
+      Tensor dout = grads[0].defined() ? grads[0] : at::zeros(v.sizes(), opt);
+      if (dout.size(2) > 1 && dout.stride(2) != 1) dout = dout.contiguous();
+      const Tensor dfinal = grads[1].defined() ? grads[1].contiguous() : Tensor();
+      out[0] = at::empty(v.sizes(), opt);
+      out[1] = at::empty(v.sizes(), opt.dtype(at::kFloat));
+      if (w.defined()) out[2] = at::empty(v.sizes(), opt);
+      if (ctx->saved_data["state"].toBool()) out[3] = at::empty({a.sequences, a.D}, opt.dtype(at::kFloat));
+      set_rows(dout, &a.dout, &a.do_batch_stride, &a.do_token_stride);
+      a.marks = ptr<float>(marks); a.dfinal_state = ptr<float>(dfinal);
+      a.dv = out[0].data_ptr(); a.dg = ptr<float>(out[1]); a.dw = ptr<void>(out[2]); a.dstate = ptr<float>(out[3]);
+      check(gdn2_recurrence_backward(&a, dtype_code(v.scalar_type()), stream_on(v)), "gdn2_recurrence_backward");
+      g_gradient_launches += recurrence_launches(a);
+    }
+    return once(std::move(out), "gated_recurrence");
+  }
+};
+
+// gated_recurrence on tensors of matching shapes and types (`offsets`: of packed sequences, or empty), and with `in_place`
+// gated_recurrence_decode. Returns (o, final state, kernels launched) or None.
+std::optional<std::tuple<Tensor, std::optional<Tensor>, int64_t>> recurrence(const Tensor& v, const Tensor& g, const std::optional<Tensor>& w,
+                                                                             const std::optional<Tensor>& state, bool want_final,
+                                                                             bool in_place, const std::vector<int64_t>& offsets) {
+  const auto dev = c10::cuda::current_device();
+  if (dtype_code(v.scalar_type()) < 0 || !unwrapped(v, v.scalar_type(), dev) || !unwrapped(g, at::kFloat, dev) || g.sizes() != v.sizes() ||
+      v.numel() == 0 || (w && (!unwrapped(*w, v.scalar_type(), dev) || w->sizes() != v.sizes())))
+    return std::nullopt;
+  const Tensor vr = as_rows(v), gr = as_rows(g), wr = w ? as_rows(*w) : Tensor();
+  if (!vr.defined() || !gr.defined() || (w && !wr.defined())) return std::nullopt;
+  const int64_t sequences = offsets.empty() ? v.size(0) : (int64_t)offsets.size() - 1;
+  std::vector<int64_t> state_shape(v.sizes().begin() + 1, v.sizes().end());
+  state_shape[0] = sequences;
+  if (state && (!unwrapped(*state, at::kFloat, dev) || !state->is_contiguous() || state->sizes() != at::IntArrayRef(state_shape)))
+    return std::nullopt;
+  const Tensor s = state ? state->view({sequences, -1}) : Tensor();
+  const bool grad = wants_grad({&vr, &gr, &wr, &s});
+  if (in_place && (grad || !state)) return std::nullopt;
+  if (grad) {
+    const auto given = [](const Tensor& t) { return t.defined() ? std::optional<Tensor>(t) : std::nullopt; };
+    auto res = Recurrence::apply(vr, gr, given(wr), given(s), offsets);
+    const int64_t launched = offsets.empty() ? 1 : (sequences + 127) / 128;
+    return std::make_tuple(res[0].view(v.sizes()), want_final ? std::optional<Tensor>(res[1].view(state_shape)) : std::nullopt, launched);
+  }
+  gdn2_recurrence_args a = recurrence_args(vr, gr, wr, offsets);
+  const auto opt = v.options().requires_grad(false);
+  Tensor o = at::empty(v.sizes(), opt);
+  std::optional<Tensor> final;
+  if (in_place) final = *state;
+  else if (want_final) final = at::empty(state_shape, opt.dtype(at::kFloat));
+  a.state = ptr<float>(s); a.o = o.data_ptr(); a.final_state = final ? ptr<float>(*final) : nullptr;
+  if (gdn2_recurrence_forward(&a, dtype_code(v.scalar_type()), stream_on(v)) != GDN2_OK) return std::nullopt;
+  return std::make_tuple(o, final, recurrence_launches(a));
+}
+
+// Matrices as the tensor-core kernels read them: rows that start on 16 bytes, elements side by side. Those that are not so are
+// copied, all in one launch. Returns whether one was.
+bool align_rows(std::vector<Tensor>& ms) {
+  std::vector<gdn2_row_copy> copies;
+  for (Tensor& t : ms) {
+    if (t.size(1) > 1 && t.stride(1) != 1) t = t.contiguous();
+    const bool one = t.size(0) == 1;
+    if ((reinterpret_cast<uintptr_t>(t.data_ptr()) & 15u) || (!one && (t.stride(0) % 8 || t.stride(0) < t.size(1)))) {
+      const int64_t pitch = (t.size(1) + 7) / 8 * 8;
+      Tensor d = at::empty({t.size(0), pitch}, t.options().requires_grad(false)).narrow(1, 0, t.size(1));
+      copies.push_back({t.data_ptr(), d.data_ptr(), t.size(0), t.size(1), one ? 0 : t.stride(0), pitch});
+      t = d;
+    }
+  }
+  if (copies.empty()) return false;
+  check(gdn2_align_rows(copies.data(), (int64_t)copies.size(), stream_on(ms[0])), "gdn2_align_rows");
+  return true;
+}
+int64_t pitch_of(const Tensor& t) { return t.size(0) > 1 ? t.stride(0) : (t.size(1) + 7) / 8 * 8; }
+gdn2_ffn_args ffn_args(const std::vector<Tensor>& in, int64_t activation) {
+  gdn2_ffn_args a{};
+  a.x = in[0].data_ptr(); a.w_gate = in[1].data_ptr(); a.w_up = in[2].data_ptr(); a.w_down = in[3].data_ptr();
+  a.tokens = in[0].size(0); a.hidden = in[0].size(1); a.out = in[3].size(0); a.inner = in[3].size(1);
+  a.x_stride = pitch_of(in[0]); a.w_gate_stride = pitch_of(in[1]); a.w_up_stride = pitch_of(in[2]); a.w_down_stride = pitch_of(in[3]);
+  a.inner_stride = (a.inner + 15) / 16 * 16;
+  a.activation = (int)activation;
+  return a;
+}
+Tensor ffn_forward(const std::vector<Tensor>& in, int64_t activation, Tensor* kept) {
+  gdn2_ffn_args a = ffn_args(in, activation);
+  const auto opt = in[0].options().requires_grad(false);
+  Tensor y = at::empty({a.tokens, a.out}, opt), h = at::empty({a.tokens, a.inner_stride}, opt);
+  if (kept) *kept = at::empty({(int64_t)gdn2_ffn_kept_bytes(a.tokens, a.inner_stride)}, opt.dtype(at::kByte));
+  a.h = h.data_ptr(); a.kept = kept ? kept->data_ptr() : nullptr; a.y = y.data_ptr(); a.y_stride = a.out;
+  check(gdn2_ffn_forward(&a, dtype_code(in[0].scalar_type()), stream_on(in[0])), "gdn2_ffn_forward");
+  return y;
+}
+
+struct FeedForward : torch::autograd::Function<FeedForward> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& wg, const Tensor& wu, const Tensor& wd, int64_t activation) {
+    std::vector<Tensor> in{x, wg, wu, wd};
+    align_rows(in);
+    Tensor kept, y = ffn_forward(in, activation, &kept);
+    ctx->save_for_backward({in[0], in[1], in[2], in[3], kept});
+    ctx->saved_data["activation"] = activation;
+    return y;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    variable_list out(5);
+    if (!grads[0].defined()) return out;
+    {
+      at::NoGradGuard no_grad;
+      const std::vector<Tensor> in(saved.begin(), saved.begin() + 4);
+      const c10::cuda::CUDAGuard device(in[0].device());
+      std::vector<Tensor> dy{grads[0]};
+      const bool copied = align_rows(dy);
+      gdn2_ffn_args a = ffn_args(in, ctx->saved_data["activation"].toInt());
+      const auto opt = in[0].options().requires_grad(false);
+      const bool dx = ctx->needs_input_grad(0), dgate = ctx->needs_input_grad(1), dup = ctx->needs_input_grad(2), ddown = ctx->needs_input_grad(3);
+      const Tensor h = at::empty({a.tokens, a.inner_stride}, opt), da = at::empty_like(h), du = at::empty_like(h);
+      if (dx) out[0] = at::empty({a.tokens, a.hidden}, opt);
+      if (dgate || dup) {
+        out[1] = at::empty({a.inner, a.hidden}, opt);
+        out[2] = at::empty({a.inner, a.hidden}, opt);
+      }
+      if (ddown) out[3] = at::empty({a.out, a.inner}, opt);
+      a.h = h.data_ptr(); a.kept = saved[4].data_ptr(); a.dy = dy[0].data_ptr(); a.dy_stride = pitch_of(dy[0]);
+      a.da = da.data_ptr(); a.du = du.data_ptr(); a.dx = ptr<void>(out[0]); a.dx_stride = a.hidden;
+      a.dw_gate = ptr<void>(out[1]); a.dw_up = ptr<void>(out[2]); a.dw_down = ptr<void>(out[3]);
+      check(gdn2_ffn_backward(&a, dtype_code(in[0].scalar_type()), stream_on(in[0])), "gdn2_ffn_backward");
+      g_gradient_launches += 1 + copied + dx + (dgate || dup) + ddown;
+      if (!dgate) out[1] = Tensor();
+      if (!dup) out[2] = Tensor();
+    }
+    return once(std::move(out), "gated_feed_forward");
+  }
+};
+
+// gated_feed_forward on tensors of matching shapes and types. Returns (y, kernels launched) or None.
+std::optional<std::tuple<Tensor, int64_t>> feed_forward(const Tensor& x, const Tensor& wg, const Tensor& wu, const Tensor& wd, int64_t activation) {
+  const auto dev = c10::cuda::current_device();
+  const auto type = x.scalar_type();
+  if ((type != at::kBFloat16 && type != at::kHalf) || !unwrapped(x, type, dev) || !unwrapped(wg, type, dev) || !unwrapped(wu, type, dev) ||
+      !unwrapped(wd, type, dev) || x.dim() < 1 || wg.dim() != 2 || wd.dim() != 2 || wu.sizes() != wg.sizes() || wd.size(1) != wg.size(0) ||
+      x.size(-1) != wg.size(1) || x.numel() == 0 || wg.numel() == 0 || wd.numel() == 0 || !(x.dim() == 2 || x.is_contiguous()))
+    return std::nullopt;
+  const Tensor rows = x.dim() == 2 ? x : x.view({-1, x.size(-1)});
+  std::vector<int64_t> shape(x.sizes().begin(), x.sizes().end());
+  shape.back() = wd.size(0);
+  if (wants_grad({&rows, &wg, &wu, &wd})) return std::make_tuple(FeedForward::apply(rows, wg, wu, wd, activation).view(shape), int64_t(2));
+  std::vector<Tensor> in{rows, wg, wu, wd};
+  const bool copied = align_rows(in);
+  return std::make_tuple(ffn_forward(in, activation, nullptr).view(shape), int64_t(2) + copied);
+}
+
 // The state of a list of parameters: where each lies, its version and its type. Equal bytes = nothing was replaced,
 // moved, converted or written to since.
 py::bytes parameter_key(const std::vector<Tensor>& params) {
@@ -302,5 +544,8 @@ PYBIND11_MODULE(_gdn2_host, m) {
   m.def("prefill_short", &prefill_short, unlocked);
   m.def("layer_decode", &layer_decode, unlocked);
   m.def("layer_prefill", &layer_prefill, unlocked);
+  m.def("recurrence", &recurrence, unlocked);
+  m.def("feed_forward", &feed_forward, unlocked);
+  m.def("gradient_launches", [] { return g_gradient_launches.load(); });
   m.def("parameter_key", &parameter_key);
 }

@@ -72,6 +72,20 @@ class _GatedRecurrence(torch.autograd.Function):
         return dv, dg, dw, dstate, None
 
 
+def _plain(v, g, w, state, want_final, in_place=False, offsets=()):
+    """The call in one native function, gradient included, where the extension takes it: ``(o, final_state | None)``, or ``None``.
+    With a status check after every call, backward passes go through Python, too."""
+    K = _cabi.kernels()
+    call = getattr(getattr(K, "host", None), "recurrence", None)
+    if call is None or K.checks_status:
+        return None
+    res = call(v, g, w, state, want_final, in_place, offsets)
+    if res is None:
+        return None
+    K.launches += res[2]
+    return res[0], res[1]
+
+
 def gated_recurrence(v, g, w=None, initial_state=None, output_final_state=False, cu_seqlens=None):
     """``h_t = exp(g_t) * h_{t-1} + w_t * v_t`` along the tokens of whole sequences; differentiable (once).
 
@@ -88,6 +102,10 @@ def gated_recurrence(v, g, w=None, initial_state=None, output_final_state=False,
     A backward pass that is captured into a CUDA graph follows PyTorch's rule for it: no other graph of the same leaves alive
     on another stream (``torch.autograd.grad`` on inputs made for the capture is safe).
     """
+    if cu_seqlens is None and v.is_cuda:
+        res = _plain(v, g, w, initial_state, output_final_state)
+        if res is not None:
+            return res
     _check_rows(v, g, w)
     B, S = v.shape[:2]
     channels = tuple(v.shape[2:])
@@ -101,6 +119,10 @@ def gated_recurrence(v, g, w=None, initial_state=None, output_final_state=False,
         _check_devices(v, initial_state)
         initial_state = initial_state.float()
     g = g.float()
+    if offsets is not None:
+        res = _plain(v, g, w, initial_state, output_final_state, offsets=offsets)
+        if res is not None:
+            return res
     if v.numel() == 0:                                 # nothing to compute: the states pass through
         final = torch.zeros(N, *channels, dtype=torch.float32, device=v.device) if initial_state is None else initial_state.clone()
         return torch.empty_like(v, memory_format=torch.contiguous_format), (final if output_final_state else None)
@@ -118,6 +140,10 @@ def gated_recurrence_decode(v, g, w, state):
     """Decode ``n`` tokens (``[B, n, ...]``), updating ``state [B, ...]`` (float32, contiguous) in place. ``w`` may be ``None``.
 
     Returns ``o [B, n, ...]`` in ``v.dtype``. No gradient."""
+    if v.is_cuda:
+        res = _plain(v, g, w, state, True, in_place=True)
+        if res is not None:
+            return res[0]
     _check_rows(v, g, w)
     B = v.shape[0]
     if tuple(state.shape) != (B, *v.shape[2:]):

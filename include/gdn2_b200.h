@@ -461,20 +461,21 @@ int gdn2_recurrence_backward(const gdn2_recurrence_args* args, int dtype, void* 
 
 /*
  * Gated feed-forward block: y = (act(x Wg^T) * (x Wu^T)) Wd^T, act SiLU or GELU (tanh form); GDN2_BF16 and GDN2_F16, sums in
- * fp32, what lies between the products (h, a = x Wg^T, u = x Wu^T and their gradients) rounded to `dtype`.
+ * fp32, what a product reads of another (h and the gradients of a = x Wg^T and u = x Wu^T) rounded to `dtype`.
  *   x [tokens, hidden]  w_gate, w_up [inner, hidden]  w_down [out, inner]  y [tokens, out]
- *   h, a, u, da, du [tokens, inner] with rows inner_stride elements apart: h is scratch of a forward call; a and u are NULL, or kept
- *   with h for a backward call; da and du are scratch of the backward call.
+ *   h, da, du [tokens, inner] with rows inner_stride elements apart (a multiple of 16): scratch, h of both calls, da and du of the
+ *   backward call. kept: NULL, or gdn2_ffn_kept_bytes(tokens, inner_stride) bytes that the forward call fills for the backward call
+ *   (a and u in 24 bits).
  * gdn2_ffn_backward: dx, (dw_gate, dw_up) and dw_down from dy; a gradient whose pointer is NULL is not computed (dw_gate and dw_up
- * together; da and du may be NULL if neither they nor dx are wanted). The weights' gradients are contiguous.
- * Row strides are in ELEMENTS. Inputs, h, a, u, da and du: rows start on 16 bytes (16-byte aligned pointers, strides that are
+ * together). The weights' gradients are contiguous.
+ * Row strides are in ELEMENTS. Inputs, h, kept, da and du: rows start on 16 bytes (16-byte aligned pointers, strides that are
  * multiples of 8), else GDN2_ERR_MISALIGNED; gdn2_align_rows copies rows that do not. y, dx and the weights' gradients may have any.
  * No counterpart in the reference, which has the token mixer alone.
  */
 enum gdn2_activation { GDN2_ACT_SILU = 0, GDN2_ACT_GELU_TANH = 1 };
 typedef struct gdn2_ffn_args {
   const void *x, *w_gate, *w_up, *w_down;
-  void *h, *a, *u;
+  void *h, *kept;
   void* y;
   const void* dy;
   void *da, *du;
@@ -484,6 +485,7 @@ typedef struct gdn2_ffn_args {
   int activation;
 } gdn2_ffn_args;
 
+size_t gdn2_ffn_kept_bytes(int64_t tokens, int64_t inner_stride);
 int gdn2_ffn_forward(const gdn2_ffn_args* args, int dtype, void* stream);
 int gdn2_ffn_backward(const gdn2_ffn_args* args, int dtype, void* stream);
 

@@ -1,9 +1,11 @@
 """The diagonal recurrence and its gradient in 64 bits, with a bound on what a float32 evaluation of it may be off by.
 
-The bound: a step multiplies by a decay that is off by at most 2 units u = 2^-24 of its value (a polynomial, its argument
-reduction and one rounding), and rounds a product and a sum; composing runs of tokens rounds two more per level. 8 u of the
-magnitude that passes a step covers them, and what has accumulated is carried on by the same decays: with the magnitudes
-m_t = a_t m_{t-1} + |x_t|, the bound is e_t = a_t e_{t-1} + 8 u m_t."""
+The bound: a step multiplies by a decay that is off by at most 4 units u = 2^-24 of its value (the approximate exponential's
+2^-22; one unit where a polynomial takes its place), and by |g| units more, because the exponential's argument g log2(e) is
+rounded (u of it, and exp turns an absolute error into a relative one). It rounds a product and a sum; composing runs of
+tokens rounds two more. 8 u of the magnitude that passes a step covers these, and what has accumulated is carried on by the same
+decays: with the magnitudes m_t = a_t m_{t-1} + |x_t|, the bound is e_t = a_t (e_{t-1} + |g_t| u m_{t-1}) + 8 u m_t. (Where
+exp(g) underflows both terms of the product with |g| are 0.)"""
 
 from __future__ import annotations
 
@@ -11,6 +13,11 @@ import torch
 
 U = 2.0**-24
 STEP = 8 * U
+
+
+def rounded(g):
+    """The error of the rounded argument of exp(g), relative."""
+    return U * g.abs().clamp(max=1e3)
 
 
 def scan(v, g, w, state, bounds=None):
@@ -26,8 +33,8 @@ def scan(v, g, w, state, bounds=None):
         m, e = h.abs(), torch.zeros_like(h)
         for t in range(lo, hi):
             a = g[b, t].exp()
-            h, m = a * h + x[b, t], a * m + x[b, t].abs()
-            e = a * e + STEP * m
+            e, m = a * (e + rounded(g[b, t]) * m), a * m + x[b, t].abs()
+            h, e = a * h + x[b, t], e + STEP * m
             o[b, t], err[b, t] = h, e
         fin[i], efin[i] = h, e
     return o, fin, err, efin
@@ -55,7 +62,7 @@ def gradients(v, g, w, state, do, dfinal, bounds=None):
             eh = e + 2 * U * mh                       # the sum do + c
             dv[b, t], ev[b, t] = dh * wd[b, t], (eh + U * dh.abs()) * wd[b, t].abs()
             dw[b, t], ew[b, t] = dh * v[b, t], (eh + U * dh.abs()) * v[b, t].abs()
-            c, m, e = a * dh, a * mh, a * e + STEP * a * mh
+            c, m, e = a * dh, a * mh, a * (e + rounded(g[b, t]) * mh) + STEP * a * mh
             dg[b, t] = c * before
             eg[b, t] = (c.abs() + e) * (eb + STEP * before.abs()) + before.abs() * e
         ds[i], es[i] = c, e

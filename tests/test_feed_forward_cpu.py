@@ -50,14 +50,13 @@ def args(**kw):
 def test_c_entry_checks():
     lib = _cabi.load_library()
     f, b = lib.gdn2_ffn_forward, lib.gdn2_ffn_backward
-    kept = dict(a=16, u=16, dy=16, da=16, du=16, dx=16)
+    kept = dict(kept=16, dy=16, da=16, du=16, dx=16)
     assert f(None, 1, None) == -1 and b(None, 1, None) == -1
     assert f(args(), 0, None) == -3 and b(args(**kept), 0, None) == -3 and f(args(), 7, None) == -3
     assert f(args(activation=2), 1, None) == -8
     for name in ("x", "w_gate", "w_up", "w_down", "h", "y"):
         assert f(args(**{name: None}), 1, None) == -1
-    assert f(args(a=16), 1, None) == -1                                    # a without u
-    for name in ("dy", "a", "u", "da", "du"):
+    for name in ("dy", "kept", "da", "du"):
         assert b(args(**{**kept, name: None}), 1, None) == -1
     assert b(args(**kept, dw_gate=16), 1, None) == -1                      # dw_gate without dw_up
     for bad in (dict(tokens=0), dict(hidden=0), dict(inner=-1), dict(out=0), dict(tokens=1 << 31), dict(x_stride=0), dict(w_down_stride=8),
@@ -65,7 +64,7 @@ def test_c_entry_checks():
         assert f(args(**bad), 1, None) == -2
         assert b(args(**kept, **bad), 1, None) == -2
     assert f(args(y_stride=7), 1, None) == -2 and b(args(**kept, dy_stride=7), 1, None) == -2 and b(args(**{**kept}, dx_stride=7), 1, None) == -2
-    for bad in (dict(x=24), dict(w_up=8), dict(x_stride=12), dict(w_down_stride=17), dict(inner_stride=17)):
+    for bad in (dict(x=24), dict(w_up=8), dict(x_stride=12), dict(w_down_stride=17), dict(inner_stride=17), dict(inner_stride=24)):
         assert f(args(**bad), 1, None) == -4
         assert b(args(**kept, **bad), 1, None) == -4
     assert b(args(**{**kept, "dy": 24}), 1, None) == -4

@@ -307,3 +307,37 @@ def test_a_long_sequence():
     # memory of 2000 tokens, 8 u a step of a magnitude of 2000 * 0.8: STEP * 2000 * 1600
     for got in (fin[0], o[0, -1]):
         assert float((got.double() - want).abs().max()) <= orc.STEP * 2000 * 1600
+
+
+@pytest.fixture
+def through_python(monkeypatch):
+    """Without the host extension every call goes through Python."""
+    from gdn2_tilelang_b200 import _cabi
+
+    monkeypatch.setattr(_cabi.kernels(), "host", None)
+
+
+@pytest.mark.parametrize("B,S,D,dtype", GRADS[:3] + GRADS[4:5])
+def test_without_the_host_extension(B, S, D, dtype, through_python):
+    test_gradients(B, S, D, dtype, True)
+    test_decode(3, D, dtype)
+    test_packed([0, 5, 5, 70], D, dtype)
+
+
+def test_once_differentiable():
+    v, g, w, s = on_gpu(*make(1, 9, 8, F32), grad=True)
+    grads = torch.autograd.grad(gdn2.gated_recurrence(v, g, w, s)[0].sum(), (v, g), create_graph=True)
+    with pytest.raises(RuntimeError, match="once"):
+        grads[1].sum().backward()
+
+
+def test_launches_are_counted():
+    from gdn2_tilelang_b200 import _cabi
+
+    K = _cabi.kernels()
+    v, g, w, s = on_gpu(*make(1, 9, 8, F32), grad=True)
+    before = K.launches
+    o, _ = gdn2.gated_recurrence(v, g, w, s)
+    assert K.launches == before + 1
+    o.sum().backward()
+    assert K.launches == before + 2
