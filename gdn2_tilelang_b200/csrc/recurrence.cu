@@ -24,6 +24,7 @@
 // The backward pass needs h_{t-1} in float32 (o is rounded, and dg = c h would keep that rounding), so the forward pass of a
 // training step leaves the state that enters every 64th token ("marks", 1/16 byte a channel and token) and the backward pass
 // composes the 64 tokens of its tile again from there.
+#include <algorithm>
 #include <atomic>
 
 #include "common.cuh"
@@ -40,10 +41,9 @@ constexpr int kC = 64;              // channels of a block
 constexpr int kMaxCluster = 8;
 constexpr int kMaxStages = 4;
 
-struct Tables {                     // packed sequences: first token and first mark of each
+struct Tables {                     // packed sequences, the longest first: which each is, its first token, its length, its first mark
   int n;
-  int tok[kMaxPacked + 1];
-  int mark[kMaxPacked + 1];
+  int seq[kMaxPacked], tok[kMaxPacked], len[kMaxPacked], mark[kMaxPacked];
 };
 
 struct Args {
@@ -103,17 +103,20 @@ template <> __device__ __forceinline__ void store_pair<__half>(__half* p, float2
 
 // Where a lane's channels lie. Fed: two neighbours, from a tile in shared memory; not fed (rows that TMA cannot read): 32 apart,
 // so that a warp's loads of single elements are whole lines.
+// Lanes behind the last channel load the last one over again, so that loads need no branch (with one, a tile's loads went out a few
+// at a time: 30 us for 3 x 1001 x 1001 float32 channels), and store nothing.
 template <bool Fed> struct Lane {
-  int c[2];
+  int c[2], last;
   bool live[2];
   __device__ __forceinline__ Lane(int group, int lane, int D) {
     c[0] = group * kC + (Fed ? 2 * lane : lane);
     c[1] = c[0] + (Fed ? 1 : 32);
+    last = D - 1;
     live[0] = c[0] < D;
     live[1] = c[1] < D;
   }
   template <typename T> __device__ __forceinline__ float2 load(const T* row) const {
-    return make_float2(live[0] ? to_f32<T>(row[c[0]]) : 0.f, live[1] ? to_f32<T>(row[c[1]]) : 0.f);
+    return make_float2(to_f32<T>(row[min(c[0], last)]), to_f32<T>(row[min(c[1], last)]));
   }
   template <typename T> __device__ __forceinline__ void store(T* row, float2 x) const {
     if constexpr (Fed) {
@@ -207,8 +210,9 @@ template <bool Packed> __device__ __forceinline__ Place place(const Args& a, con
   if constexpr (Packed) {
     p.batch = 0;
     p.start = tb.tok[p.seq];
-    p.len = tb.tok[p.seq + 1] - p.start;
+    p.len = tb.len[p.seq];
     p.mark = tb.mark[p.seq];
+    p.seq = tb.seq[p.seq];
   } else {
     p.batch = p.seq;
     p.start = 0;
@@ -595,33 +599,44 @@ int active_clusters(int per_sm, int cl) {
 // How a scan is laid out: warps of a block, blocks of a cluster, stages of a block's feed: the quickest by this account of it. A
 // cluster takes the tiles of its row a round at a time. A round lasts at least as long as the chain of composing and exchanging it,
 // and as all that the blocks at work move in it takes at the copy rate (6500 bytes a nanosecond). Rows that find no place wait for
-// the next wave; a wave starts and ends in 3 us. Chains as measured on one row, in us: forward 0.95 with 8 warps, 1.45 with 16,
+// the next wave; a wave starts and ends in 3 us. Packed sequences are of many lengths: the longest alone, all at the copy rate, or
+// all one after another in the places there are, whichever is longest (ten of 16037 tokens together, 2048 channels: clusters of 1
+// 88 us, the longest sequence's chain; as chosen 62). Chains as measured on one row, in us: forward 0.95 with 8 warps, 1.45 with 16,
 // backward 1.85 and 2.8, in clusters 0.2 and 0.02 a block more. Against measurements, forward, bf16, in us: 2 x 4096 x 2048 channels,
 // 8 warps, clusters of 1, 2, 4: 64, 43, 29 and 65, 44, 32; 16 x 4096 x 1024, 8 and 16 warps: 106, 111 and 119, 112.
 struct Layout {
   int warps, cluster, stages;
   size_t smem;
 };
-Layout layout(int64_t rows, int64_t tokens, size_t token_bytes, size_t traffic, bool fed, bool back, int warps_most) {
+Layout layout(int64_t rows, int64_t longest, double average, size_t token_bytes, size_t traffic, bool fed, bool back, int warps_most) {
   Layout best{};
   double least = 0;
   for (int W = 8; W <= warps_most; W *= 2) {
     const int tile = W * kR;
     const size_t stage = fed ? tile * token_bytes : 0;
     const size_t fixed = (size_t)(back ? 2 * W : W + 1) * 512 + 512;          // a block's Shared
-    const int64_t tiles = (tokens + tile - 1) / tile;
+    const int64_t tiles = (longest + tile - 1) / tile;
     for (int cl = 1; cl <= kMaxCluster && (cl == 1 || cl <= tiles); ++cl) {
       const size_t slots = (size_t)2 * cl * 32 * sizeof(float4);
       for (int per_sm = W > 8 ? 1 : back ? 2 : 3; per_sm >= 1; --per_sm) {     // the kernels' launch bounds, or fewer blocks and more stages
         const size_t room = (size_t)228 * 1024 / per_sm - 1024 - fixed - slots;
         if (room < 2 * stage) continue;
         const int64_t most = active_clusters(per_sm, cl);
-        const double chain = (back ? (W > 8 ? 2.8 : 1.85) : (W > 8 ? 1.45 : 0.95)) + (cl > 1 ? 0.2 + 0.02 * cl : 0.0);
-        auto wave = [&](int64_t clusters) {
-          const double bytes = (double)clusters * cl * tile * traffic / 6.5e6;
-          return clusters == 0 ? 0.0 : (double)((tiles + cl - 1) / cl) * (bytes > chain ? bytes : chain) + 3.0;
-        };
-        const double cost = (double)(rows / most) * wave(most) + wave(rows % most);
+        const double chain = (back ? (W > 8 ? 2.8 : 1.85) : (W > 8 ? 1.45 : 0.95)) + (cl > 1 ? 0.2 + 0.02 * cl : 0.0) + (fed ? 0.0 : 1.2);
+        const int64_t rounds = (tiles + cl - 1) / cl;
+        double cost;
+        if (average == (double)longest) {
+          auto wave = [&](int64_t clusters) {
+            const double bytes = (double)clusters * cl * tile * traffic / 6.5e6;
+            return clusters == 0 ? 0.0 : rounds * (bytes > chain ? bytes : chain) + 3.0;
+          };
+          cost = (double)(rows / most) * wave(most) + wave(rows % most);
+        } else {                                       // the longest first, and the others after one another in the places that are left
+          const double bytes = (double)rows * average * traffic / 6.5e6, mean = average / (tile * cl) + 0.5;
+          const double alone = rounds * chain + 3.0, shared = (double)rows / most * (mean * chain + 3.0);
+          cost = bytes > alone ? bytes : alone;
+          cost = (cost > shared ? cost : shared) + 3.0;
+        }
         if (best.warps == 0 || cost < 0.99 * least) {
           least = cost;
           best.warps = W;
@@ -651,13 +666,13 @@ template <typename T> constexpr CUtensorMapDataType map_type() {
 }
 
 template <typename T, bool Gate, bool Packed, bool Fed>
-int launch_scan(const Args& a0, const Tables& tb, int64_t longest, bool backward, cudaStream_t st) {
+int launch_scan(const Args& a0, const Tables& tb, int64_t longest, double average, bool backward, cudaStream_t st) {
   Args a = a0;
   a.groups = (a.D + kC - 1) / kC;
   const int64_t rows = (int64_t)a.sequences * a.groups, batches = Packed ? 1 : a.sequences;
   const size_t token = kC * (4 + sizeof(T) * (1 + Gate + backward));                                   // read
   const size_t written = kC * (backward ? 4 + sizeof(T) * (1 + Gate) : sizeof(T));
-  const Layout l = layout(rows, longest, token, token + written, Fed, backward, Fed ? 16 : 8);
+  const Layout l = layout(rows, longest, average, token, token + written, Fed, backward, Fed ? 16 : 8);
   if (rows * l.cluster > 2147483647LL) return GDN2_ERR_BAD_SHAPE;
   Maps maps{};
   const int tile = l.warps * kR;
@@ -699,27 +714,34 @@ int launch_all(const Args& a, const int64_t* cu, bool backward, cudaStream_t st)
       GDN2_CUDA_TRY(cudaGetLastError());
       return GDN2_OK;
     }
-    return launch_scan<T, Gate, false, (VEC > 1)>(a, none, a.S, backward, st);
+    return launch_scan<T, Gate, false, (VEC > 1)>(a, none, a.S, (double)a.S, backward, st);
   }
   int64_t mark = 0;
   for (int i0 = 0; i0 < a.sequences; i0 += kMaxPacked) {
     Tables tb;
     tb.n = a.sequences - i0 < kMaxPacked ? a.sequences - i0 : kMaxPacked;
-    int64_t longest = 0;
-    for (int i = 0; i <= tb.n; ++i) {
-      tb.tok[i] = (int)cu[i0 + i];
-      tb.mark[i] = (int)mark;
-      if (i < tb.n) {
-        const int64_t len = cu[i0 + i + 1] - cu[i0 + i];
-        longest = len > longest ? len : longest;
-        mark += (len + kMark - 1) / kMark;
-      }
+    int order[kMaxPacked], marks[kMaxPacked];
+    for (int i = 0; i < tb.n; ++i) {
+      order[i] = i;
+      marks[i] = (int)mark;
+      mark += (cu[i0 + i + 1] - cu[i0 + i] + kMark - 1) / kMark;
     }
+    auto len = [&](int i) { return cu[i0 + i + 1] - cu[i0 + i]; };
+    std::sort(order, order + tb.n, [&](int x, int y) { return len(x) != len(y) ? len(x) > len(y) : x < y; });
+    for (int k = 0; k < tb.n; ++k) {
+      const int i = order[k];
+      tb.seq[k] = i;
+      tb.tok[k] = (int)cu[i0 + i];
+      tb.len[k] = (int)len(i);
+      tb.mark[k] = marks[i];
+    }
+    const int64_t longest = len(order[0]);
+    const double average = (double)(cu[i0 + tb.n] - cu[i0]) / tb.n;
     Args part = a;
     part.sequences = tb.n;
     if (a.first) part.first = a.first + (int64_t)i0 * a.D;
     if (a.last) part.last = a.last + (int64_t)i0 * a.D;
-    const int rc = launch_scan<T, Gate, true, (VEC > 1)>(part, tb, longest, backward, st);
+    const int rc = launch_scan<T, Gate, true, (VEC > 1)>(part, tb, longest, average, backward, st);
     if (rc != GDN2_OK) return rc;
   }
   return GDN2_OK;
