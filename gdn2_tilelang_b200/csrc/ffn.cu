@@ -24,6 +24,7 @@
 // Few tokens (skinny_kernel): the work is reading the weights once. They take the 128-row side of the product, the tokens
 // the narrow one, and the reduction of a tile is cut over the blocks of a cluster so that every SM reads; the blocks' partial
 // sums meet in distributed shared memory, added in the order of the blocks.
+#include "clusters.cuh"
 #include "common.cuh"
 #include "tc_utils.cuh"
 #include "tensor_map.cuh"
@@ -43,7 +44,7 @@ constexpr uint32_t kWaitCode = 1u << 28;
 
 enum Kind { kPlain = 0, kGated = 1, kGatedBackward = 2 };
 
-// Stages that fit beside a kind's staging buffers: one chunk a warp, three in and out for the backward epilogue.
+// Stages that fit beside a kind's staging buffers: one chunk a warp; for the backward epilogue 6 KB in and 6 KB out.
 template <int K> __host__ __device__ constexpr int stages() { return K == kGatedBackward ? 4 : 6; }
 template <int K> __host__ __device__ constexpr int staging_bytes() { return kEpiWarps * kChunkBytes * (K == kGatedBackward ? 3 : 1); }
 template <int K> constexpr size_t smem_bytes() { return (size_t)stages<K>() * kStageBytes + staging_bytes<K>() + 1024; }
@@ -58,7 +59,7 @@ struct Problem {
   int tiles_m, tiles_n;
   int split_m;                  // > 0: tiles from this one on take a[1] and out[1], their rows counted from there (dWg, dWu)
   int M, N;                     // rows and columns of the result (of one part)
-  int save, gelu;               // kGated: a and u are kept; kGatedBackward: h is wanted
+  int save;                     // kGated: a and u are kept; kGatedBackward: h is wanted
   void* plain_out[2];           // results whose rows do not start on 16 bytes are stored by threads
   int64_t out_stride;
 };
@@ -144,18 +145,20 @@ template <typename T> __host__ __device__ constexpr uint32_t idesc_of(bool a_mn,
 
 // act(a) and, where wanted, act'(a). Both are a times a logistic function: silu s(a), gelu's tanh form s(2 z) with
 // z = sqrt(2 / pi) (a + 0.044715 a^3). Beyond |a| = 16 the latter is 0 or 1 to 32 bits; z stops there so that a^3 stays finite.
+// (A template argument: with a branch on it inside the epilogue's loops the backward one took twice as long as its products.)
 // The exponential and the reciprocal are the approximate instructions: 2^-21, against results of 11 bits at most.
 __device__ __forceinline__ float logistic(float x) { return __fdividef(1.f, 1.f + __expf(-x)); }
-template <bool Slope> __device__ __forceinline__ float activate(float a, int gelu, float& slope) {
-  if (gelu) {
+template <bool Gelu, bool Slope> __device__ __forceinline__ float activate(float a, float& slope) {
+  if constexpr (Gelu) {
     const float c = 0.7978845608028654f, t = fminf(fmaxf(a, -16.f), 16.f), t2 = t * t;
     const float s = logistic(2.f * c * t * fmaf(0.044715f, t2, 1.f));
     if constexpr (Slope) slope = fmaf(2.f * c * t * s * (1.f - s), fmaf(3.f * 0.044715f, t2, 1.f), s);
     return a * s;
+  } else {
+    const float s = logistic(a);
+    if constexpr (Slope) slope = s * fmaf(a, 1.f - s, 1.f);
+    return a * s;
   }
-  const float s = logistic(a);
-  if constexpr (Slope) slope = s * fmaf(a, 1.f - s, 1.f);
-  return a * s;
 }
 
 // ---------------------------------------------------------------- the epilogue's chunks: 32 rows of 64 columns, swizzled
@@ -208,14 +211,32 @@ __device__ __forceinline__ void put_upper(char* chunk, int lane, int first, cons
                    upper16(b[8 * j + 6], b[8 * j + 7]));
 }
 __device__ __forceinline__ uint32_t lower_at(int lane, int j) { return lane * 64 + ((j ^ ((lane >> 1) & 3)) * 16); }
-__device__ __forceinline__ void get_kept(const char* upper, const uint4 (&lower)[4], int lane, int first, float (&x)[32]) {
+// The backward epilogue's pieces are 32 columns: rows of 64 bytes of 16-bit elements (swizzled as TMA does it with rows of 64) and
+// of 32 bytes of the lower planes (with rows of 32).
+__device__ __forceinline__ uint32_t row64_at(int lane, int j) { return lane * 64 + ((j ^ ((lane >> 1) & 3)) * 16); }
+template <typename T> __device__ __forceinline__ void put_row64(char* piece, int lane, const float (&x)[32]) {
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    const uint4 r = *reinterpret_cast<const uint4*>(upper + lane * 128 + (((first / 8 + j) ^ (lane & 7)) * 16));
-    const uint32_t h[4] = {r.x, r.y, r.z, r.w}, *l = reinterpret_cast<const uint32_t*>(&lower[first / 16 + j / 2]) + 2 * (j & 1);
+    uint4 r;
+    r.x = pack2<T>(x[8 * j], x[8 * j + 1]); r.y = pack2<T>(x[8 * j + 2], x[8 * j + 3]);
+    r.z = pack2<T>(x[8 * j + 4], x[8 * j + 5]); r.w = pack2<T>(x[8 * j + 6], x[8 * j + 7]);
+    *reinterpret_cast<uint4*>(piece + row64_at(lane, j)) = r;
+  }
+}
+__device__ __forceinline__ void get_kept(const char* upper, const char* lower, int lane, float (&x)[32]) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i)       // two bytes of the upper plane, one of the lower
-      x[8 * j + i] = __uint_as_float(__byte_perm(h[i / 2], l[i / 4], (i & 1 ? 0x3200 : 0x1000) | (4 + (i & 3)) << 4) & 0xffffff00u);
+  for (int half = 0; half < 2; ++half) {
+    const uint4 lo = *reinterpret_cast<const uint4*>(lower + lane * 32 + ((half ^ ((lane >> 2) & 1)) * 16));
+    const uint32_t l[4] = {lo.x, lo.y, lo.z, lo.w};
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const uint4 r = *reinterpret_cast<const uint4*>(upper + row64_at(lane, 2 * half + j));
+      const uint32_t h[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+      for (int i = 0; i < 8; ++i)     // two bytes of the upper plane, one of the lower
+        x[16 * half + 8 * j + i] =
+            __uint_as_float(__byte_perm(h[i / 2], l[2 * j + i / 4], (i & 1 ? 0x3200 : 0x1000) | (4 + (i & 3)) << 4) & 0xffffff00u);
+    }
   }
 }
 // A warp's chunk to rows row.., columns col.. of the result; what lies outside is dropped.
@@ -270,7 +291,7 @@ __device__ __forceinline__ void tile_at(const Problem& p, int i, int& m, int& n)
   n = (i - b * per) / rows;
 }
 
-template <typename T, int K, bool A_MN, bool B_MN>
+template <typename T, int K, bool A_MN, bool B_MN, bool Gelu>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 product_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Problem p, uint32_t* status) {
   constexpr int S = stages<K>();
@@ -375,22 +396,22 @@ product_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Proble
     const uint32_t lanes = (uint32_t)(quad * 32) << 16;
     const uint32_t taken0 = in_block(tc::smem_u32(&sh.taken[0]), 0), taken1 = in_block(tc::smem_u32(&sh.taken[1]), 0);
     int buf = 0, phase = 0;
-    int loads = 0;                                    // kGatedBackward: chunks loaded so far
-    auto load_chunk = [&](int i, int c) {             // chunk c (0, 1) of this warp's half of tile i: a and u
+    int loads = 0;                                    // kGatedBackward: pieces loaded so far
+    auto load_piece = [&](int i, int c) {             // 32 columns of a and u, piece c of this warp's half of tile i
       if (i >= tiles) return;
       int m, n;
       tile_at(p, i, m, n);
       if (lane == 0) {
-        const int row = m * kTile + rank * kBlockRows + quad * 32, col = n * kTile + half * 128 + c * kChunk16;
+        const int row = m * kTile + rank * kBlockRows + quad * 32, col = n * kTile + half * 128 + c * 32;
         const uint32_t bar = tc::smem_u32(&sh.loaded[ew]), at = tc::smem_u32(chunk);
-        tc::mbar_expect_tx(&sh.loaded[ew], 3 * kChunkBytes);
+        tc::mbar_expect_tx(&sh.loaded[ew], 6144);
         tma_load(at, &maps.kept[0], col, row, bar);
-        tma_load(at + kChunkBytes, &maps.kept[1], col, row, bar);
-        tma_load(at + 2 * kChunkBytes, &maps.kept[2], col, row, bar);
-        tma_load(at + 2 * kChunkBytes + kChunkBytes / 2, &maps.kept[3], col, row, bar);
+        tma_load(at + 2048, &maps.kept[1], col, row, bar);
+        tma_load(at + 4096, &maps.kept[2], col, row, bar);
+        tma_load(at + 5120, &maps.kept[3], col, row, bar);
       }
     };
-    if constexpr (K == kGatedBackward) load_chunk(pair, 0);
+    if constexpr (K == kGatedBackward) load_piece(pair, 0);
     for (int i = pair; i < tiles; i += pairs) {
       int m, n;
       tile_at(p, i, m, n);
@@ -433,7 +454,7 @@ product_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Proble
 #pragma unroll
               for (int j = 0; j < 32; ++j) {
                 float none;
-                a[j] = activate<false>(a[j], p.gelu, none) * u[j];
+                a[j] = activate<Gelu, false>(a[j], none) * u[j];
               }
               put_row<T>(chunk, lane, 32 * q, a);
             } else {
@@ -459,48 +480,44 @@ product_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Proble
           store_chunk<T>(chunk + kChunkBytes / 2, &maps.kept[3], nullptr, 0, row, col, p.M, p.N, lane);
         }
       } else {
+        // a piece's a and u go to registers, the next piece's are asked for, and only then the work on them begins: the load's latency
+        // and the stores' are both behind it (loading after the stores of the piece before: 250 us instead of 209 for 8192 x 2048 x 5632)
         bool ok = true;
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          const int at = half * 128 + c * kChunk16;
+        char* out = chunk + 6144;
+#pragma unroll 1
+        for (int c = 0; c < 4; ++c) {
           ok = tc::mbar_wait_warp(&sh.loaded[ew], loads & 1, &sh.abort, status, kWaitCode);
           if (!ok) break;
           ++loads;
-          uint4 alow[4], ulow[4];
-          char* third = chunk + 2 * kChunkBytes;
+          float d[32], a[32], u[32];
+          tc::tmem_ld32(acc + half * 128 + 32 * c, d);
+          get_kept(chunk, chunk + 4096, lane, a);
+          get_kept(chunk + 2048, chunk + 5120, lane, u);
+          __syncwarp();
+          if (c < 3) load_piece(i, c + 1); else load_piece(i + pairs, 0);
+          tc::tmem_ld_wait();
+          float h[32];
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            alow[j] = *reinterpret_cast<const uint4*>(third + lower_at(lane, j));
-            ulow[j] = *reinterpret_cast<const uint4*>(third + kChunkBytes / 2 + lower_at(lane, j));
+          for (int j = 0; j < 32; ++j) {
+            float slope;
+            const float act = activate<Gelu, true>(a[j], slope);
+            h[j] = act * u[j];
+            a[j] = d[j] * u[j] * slope;
+            u[j] = d[j] * act;
           }
-          __syncwarp();                               // h takes the lower planes' place
-#pragma unroll
-          for (int q = 0; q < 2; ++q) {
-            float d[32], a[32], u[32];
-            tc::tmem_ld32(acc + at + 32 * q, d);
-            get_kept(chunk, alow, lane, 32 * q, a);
-            get_kept(chunk + kChunkBytes, ulow, lane, 32 * q, u);
-            tc::tmem_ld_wait();
-            float h[32];
-#pragma unroll
-            for (int j = 0; j < 32; ++j) {
-              float slope;
-              const float act = activate<true>(a[j], p.gelu, slope);
-              h[j] = act * u[j];
-              a[j] = d[j] * u[j] * slope;
-              u[j] = d[j] * act;
-            }
-            put_row<T>(chunk, lane, 32 * q, a);
-            put_row<T>(chunk + kChunkBytes, lane, 32 * q, u);
-            put_row<T>(third, lane, 32 * q, h);
-          }
-          const int col = n * kTile + at;
-          store_chunk<T>(chunk, &maps.out[0], nullptr, 0, row, col, p.M, p.N, lane);
-          store_chunk<T>(chunk + kChunkBytes, &maps.out[1], nullptr, 0, row, col, p.M, p.N, lane);
-          if (p.save) store_chunk<T>(third, &maps.out[2], nullptr, 0, row, col, p.M, p.N, lane);
-          tc::fence_async_smem();                     // a chunk outside the result was not stored: order its rewriting all the same
           chunk_free(lane);
-          if (c == 0) load_chunk(i, 1); else load_chunk(i + pairs, 0);
+          put_row64<T>(out, lane, a);
+          put_row64<T>(out + 2048, lane, u);
+          put_row64<T>(out + 4096, lane, h);
+          tc::fence_async_smem();
+          __syncwarp();
+          const int col = n * kTile + half * 128 + 32 * c;
+          if (lane == 0 && row < p.M && col < p.N) {
+            tma_store(&maps.out[0], col, row, tc::smem_u32(out));
+            tma_store(&maps.out[1], col, row, tc::smem_u32(out + 2048));
+            if (p.save) tma_store(&maps.out[2], col, row, tc::smem_u32(out + 4096));
+            tc::bulk_commit();
+          }
         }
         if (!ok) break;
       }
@@ -541,7 +558,7 @@ struct Skinny {
 };
 
 template <typename T, bool Gated>
-__global__ void __launch_bounds__(kSkinnyThreads, 1) skinny_kernel(const __grid_constant__ SkinnyMaps maps, const __grid_constant__ Skinny p,
+__global__ void __launch_bounds__(kSkinnyThreads, 2) skinny_kernel(const __grid_constant__ SkinnyMaps maps, const __grid_constant__ Skinny p,
                                                                   uint32_t* status) {
   extern __shared__ __align__(1024) char smem_raw[];
   __shared__ Shared sh;
@@ -552,6 +569,14 @@ __global__ void __launch_bounds__(kSkinnyThreads, 1) skinny_kernel(const __grid_
   const int k0 = (int)((int64_t)p.steps * rank / CL), k1 = (int)((int64_t)p.steps * (rank + 1) / CL);
   constexpr int kWeightBytes = (Gated ? 2 : 1) * kOperandBytes;
   const int token_bytes = p.width * kStep * 2;
+  auto fetch = [&](int k, int s) {
+    const uint32_t bar = tc::smem_u32(&sh.full[s]), dst = tc::smem_u32(ring + s * p.stage_bytes);
+    tc::mbar_expect_tx(&sh.full[s], kWeightBytes + token_bytes);
+    tma_load(dst, &maps.w[0], k * kStep, row0, bar);
+    if constexpr (Gated) tma_load(dst + kOperandBytes, &maps.w[1], k * kStep, row0, bar);
+    tma_load(dst + kWeightBytes, &maps.x, k * kStep, 0, bar);
+  };
+  const int first = min(p.stages, k1 - k0);           // stages that are asked for before anything else
   if (wid == 0 && lane == 0) {
     for (int i = 0; i < p.stages; ++i) {
       tc::mbar_init(&sh.full[i], 1);
@@ -560,6 +585,8 @@ __global__ void __launch_bounds__(kSkinnyThreads, 1) skinny_kernel(const __grid_
     tc::mbar_init(&sh.done[0], 1);
     sh.abort = 0;
     tc::mbar_init_fence();
+    tc::fence_async_smem();
+    for (int i = 0; i < first; ++i) fetch(k0 + i, i);
   }
   if (wid == 2) tc::tmem_alloc(&sh.tmem, 128);
   tc::tc_fence_before_sync();
@@ -569,14 +596,10 @@ __global__ void __launch_bounds__(kSkinnyThreads, 1) skinny_kernel(const __grid_
 
   if (wid == 0) {
     if (lane == 0) {
-      int s = 0, phase = 0;
-      for (int k = k0; k < k1; ++k) {
-        if (!tc::mbar_wait(&sh.empty[s], phase ^ 1, &sh.abort, status, kWaitCode)) break;
-        const uint32_t bar = tc::smem_u32(&sh.full[s]), dst = tc::smem_u32(ring + s * p.stage_bytes);
-        tc::mbar_expect_tx(&sh.full[s], kWeightBytes + token_bytes);
-        tma_load(dst, &maps.w[0], k * kStep, row0, bar);
-        if constexpr (Gated) tma_load(dst + kOperandBytes, &maps.w[1], k * kStep, row0, bar);
-        tma_load(dst + kWeightBytes, &maps.x, k * kStep, 0, bar);
+      int s = first == p.stages ? 0 : first, phase = 0;
+      for (int k = k0 + first; k < k1; ++k) {
+        if (!tc::mbar_wait(&sh.empty[s], phase, &sh.abort, status, kWaitCode)) break;
+        fetch(k, s);
         if (++s == p.stages) { s = 0; phase ^= 1; }
       }
     }
@@ -626,40 +649,56 @@ __global__ void __launch_bounds__(kSkinnyThreads, 1) skinny_kernel(const __grid_
   __syncthreads();
   after_a_failure(&sh.abort);
   if (CL > 1) cluster_sync();
-  // every block finishes the tokens n = rank, rank + CL, ...: a thread a weight row, the blocks' sums in their order
+  // every block finishes its share of the tile's rows for all tokens: the blocks' sums in their order
   {
-    const int r = tid & (kBlockRows - 1), row = row0 + r;
+    const int q0 = 32 * rank / CL, share = 32 * (rank + 1) / CL - q0;         // in groups of four rows
     const uint32_t part = tc::smem_u32(ring);
-    if (row < p.rows)
-      for (int n = rank + CL * (tid / kBlockRows); n < p.tokens; n += CL * (kSkinnyThreads / kBlockRows)) {
-        float v[2] = {0.f, 0.f};
-        for (int b = 0; b < CL; ++b) {
-          const uint32_t peer = CL > 1 ? in_block(part, b) : part;
+    uint32_t peer[kMaxSplit];
 #pragma unroll
-          for (int g = 0; g < (Gated ? 2 : 1); ++g) {
-            float x;
-            asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(x) : "r"(peer + ((g * p.width + n) * kBlockRows + r) * 4) : "memory");
-            v[g] += x;
+    for (int b = 0; b < kMaxSplit; ++b) peer[b] = in_block(part, b < CL ? b : rank);
+    for (int i = tid; i < p.tokens * share; i += kSkinnyThreads) {
+      const int n = i / share, r = 4 * (q0 + i - n * share), row = row0 + r;
+      if (row >= p.rows) continue;
+      float4 x[Gated ? 2 : 1][kMaxSplit], sum[2] = {};
+#pragma unroll
+      for (int g = 0; g < (Gated ? 2 : 1); ++g)
+#pragma unroll
+        for (int b = 0; b < kMaxSplit; ++b)
+          if (b < CL) {
+            float4& f = x[g][b];
+            asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(f.x), "=f"(f.y), "=f"(f.z), "=f"(f.w)
+                         : "r"(peer[b] + ((g * p.width + n) * kBlockRows + r) * 4) : "memory");
           }
-        }
-        T* out = static_cast<T*>(p.out) + (int64_t)n * p.out_stride + row;
+#pragma unroll
+      for (int g = 0; g < (Gated ? 2 : 1); ++g)
+#pragma unroll
+        for (int b = 0; b < kMaxSplit; ++b)
+          if (b < CL) {
+            sum[g].x += x[g][b].x; sum[g].y += x[g][b].y; sum[g].z += x[g][b].z; sum[g].w += x[g][b].w;
+          }
+      const float *v0 = &sum[0].x, *v1 = &sum[1].x;
+      T* out = static_cast<T*>(p.out) + (int64_t)n * p.out_stride + row;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        if (row + k >= p.rows) continue;
         if constexpr (Gated) {
           float none;
-          *out = from_f32<T>(activate<false>(v[0], p.gelu, none) * v[1]);
+          out[k] = from_f32<T>((p.gelu ? activate<true, false>(v0[k], none) : activate<false, false>(v0[k], none)) * v1[k]);
           if (p.kept) {
-            const Planes k = planes(p.kept, p.tokens, p.kept_stride);
-            const int64_t e = (int64_t)n * p.kept_stride + row;
+            const Planes pl = planes(p.kept, p.tokens, p.kept_stride);
+            const int64_t e = (int64_t)n * p.kept_stride + row + k;
 #pragma unroll
             for (int g = 0; g < 2; ++g) {
-              const uint32_t b = round24(v[g]);
-              k.upper[g][e] = (uint16_t)(b >> 16);
-              k.lower[g][e] = (uint8_t)(b >> 8);
+              const uint32_t b = round24(g ? v1[k] : v0[k]);
+              pl.upper[g][e] = (uint16_t)(b >> 16);
+              pl.lower[g][e] = (uint8_t)(b >> 8);
             }
           }
         } else {
-          *out = from_f32<T>(v[0]);
+          out[k] = from_f32<T>(v0[k]);
         }
       }
+    }
   }
   __syncthreads();
   if (CL > 1) cluster_sync();                         // no block leaves while another reads its sums
@@ -692,29 +731,30 @@ __global__ void __launch_bounds__(256) align_rows_kernel(const __grid_constant__
 
 // ---------------------------------------------------------------- host side
 
-// a [rows, cols] matrix of 16-bit elements with rows `stride` elements apart, in boxes of box_rows x 64
+// a [rows, cols] matrix of 16-bit elements with rows `stride` elements apart, in boxes of box_rows x 64 (or 32) columns, swizzled over
+// the box's row
 struct Matrix {
   const void* p;
   int64_t rows, cols, stride;
 };
-bool make_map(CUtensorMap* map, const Matrix& m, int box_rows, CUtensorMapDataType type, int size) {
+bool make_map(CUtensorMap* map, const Matrix& m, int box_rows, CUtensorMapDataType type, int size, int cols = 64) {
   const EncodeTiled fn = encode_tiled();
   if (!fn) return false;
   const cuuint64_t dims[2] = {(cuuint64_t)m.cols, (cuuint64_t)m.rows}, strides[1] = {(cuuint64_t)m.stride * size};
-  const cuuint32_t box[2] = {64, (cuuint32_t)box_rows}, unit[2] = {1, 1};
+  const cuuint32_t box[2] = {(cuuint32_t)cols, (cuuint32_t)box_rows}, unit[2] = {1, 1};
   return fn(map, type, 2, const_cast<void*>(m.p), dims, strides, box, unit, CU_TENSOR_MAP_INTERLEAVE_NONE,
-            size == 2 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            cols * size == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : cols * size == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_32B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
-bool make_map(CUtensorMap* map, const Matrix& m, int box_rows, int dtype) {
-  return make_map(map, m, box_rows, dtype == GDN2_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2);
+bool make_map(CUtensorMap* map, const Matrix& m, int box_rows, int dtype, int cols = 64) {
+  return make_map(map, m, box_rows, dtype == GDN2_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, cols);
 }
 // the planes of a kept buffer
-bool make_kept_maps(CUtensorMap (&maps)[4], void* kept, const Matrix& h) {
+bool make_kept_maps(CUtensorMap (&maps)[4], void* kept, const Matrix& h, int cols) {
   const Planes k = planes(kept, h.rows, h.stride);
   for (int g = 0; g < 2; ++g)
-    if (!make_map(&maps[g], Matrix{k.upper[g], h.rows, h.cols, h.stride}, 32, CU_TENSOR_MAP_DATA_TYPE_UINT16, 2) ||
-        !make_map(&maps[2 + g], Matrix{k.lower[g], h.rows, h.cols, h.stride}, 32, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1))
+    if (!make_map(&maps[g], Matrix{k.upper[g], h.rows, h.cols, h.stride}, 32, CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, cols) ||
+        !make_map(&maps[2 + g], Matrix{k.lower[g], h.rows, h.cols, h.stride}, 32, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, cols))
       return false;
   return true;
 }
@@ -723,11 +763,11 @@ bool aligned_rows(const Matrix& m) { return (reinterpret_cast<uintptr_t>(m.p) & 
 int steps_of(int64_t k) { return (int)((k + kStep - 1) / kStep); }
 int tiles_of(int64_t n, int tile) { return (int)((n + tile - 1) / tile); }
 
-template <typename T, int K, bool A_MN, bool B_MN>
+template <typename T, int K, bool A_MN, bool B_MN, bool Gelu = false>
 int launch_product(const Maps& maps, const Problem& p, cudaStream_t st) {
   uint32_t* status = device_status_word();
   if (!status) return record_cuda_error(cudaGetLastError());
-  auto kernel = product_kernel<T, K, A_MN, B_MN>;
+  auto kernel = product_kernel<T, K, A_MN, B_MN, Gelu>;
   GDN2_CUDA_TRY(ensure_dynamic_smem(reinterpret_cast<const void*>(kernel), smem_bytes<K>()));
   const int tiles = p.tiles_m * p.tiles_n, pairs = device_sm_count() / 2;
   kernel<<<2 * (tiles < pairs ? tiles : pairs), kThreads, smem_bytes<K>(), st>>>(maps, p, status);
@@ -749,15 +789,14 @@ int gated_forward(const Matrix& x, const Matrix& wg, const Matrix& wu, const Mat
   GDN2_MAP(maps.b[0], wg, kBlockRows);
   GDN2_MAP(maps.b[1], wu, kBlockRows);
   GDN2_MAP(maps.out[0], h, 32);
-  if (kept && !make_kept_maps(maps.kept, kept, h)) return GDN2_ERR_UNSUPPORTED;
+  if (kept && !make_kept_maps(maps.kept, kept, h, kChunk16)) return GDN2_ERR_UNSUPPORTED;
   p.steps[0] = steps_of(x.cols);
   p.tiles_m = tiles_of(x.rows, kTile);
   p.tiles_n = tiles_of(wg.rows, kBlockRows);
   p.M = (int)x.rows;
   p.N = (int)wg.rows;
   p.save = kept != nullptr;
-  p.gelu = gelu;
-  return launch_product<T, kGated, false, false>(maps, p, st);
+  return gelu ? launch_product<T, kGated, false, false, true>(maps, p, st) : launch_product<T, kGated, false, false, false>(maps, p, st);
 }
 
 // da, du (and h) from dy, Wd and what was kept of a, u
@@ -768,18 +807,17 @@ int gated_backward(const Matrix& dy, const Matrix& wd, void* kept, const Matrix&
   Problem p{};
   GDN2_MAP(maps.a[0], dy, kBlockRows);
   GDN2_MAP(maps.b[0], wd, kStep);
-  if (!make_kept_maps(maps.kept, kept, h)) return GDN2_ERR_UNSUPPORTED;
-  GDN2_MAP(maps.out[0], da, 32);
-  GDN2_MAP(maps.out[1], du, 32);
-  GDN2_MAP(maps.out[2], h, 32);
+  if (!make_kept_maps(maps.kept, kept, h, 32) || !make_map(&maps.out[0], da, 32, dtype, 32) || !make_map(&maps.out[1], du, 32, dtype, 32) ||
+      !make_map(&maps.out[2], h, 32, dtype, 32))
+    return GDN2_ERR_UNSUPPORTED;
   p.save = want_h;
   p.steps[0] = steps_of(dy.cols);
   p.tiles_m = tiles_of(dy.rows, kTile);
   p.tiles_n = tiles_of(wd.cols, kTile);
   p.M = (int)dy.rows;
   p.N = (int)wd.cols;
-  p.gelu = gelu;
-  return launch_product<T, kGatedBackward, false, true>(maps, p, st);
+  return gelu ? launch_product<T, kGatedBackward, false, true, true>(maps, p, st)
+              : launch_product<T, kGatedBackward, false, true, false>(maps, p, st);
 }
 
 int set_out(Maps& maps, Problem& p, int part, const Matrix& out, int dtype) {
@@ -845,21 +883,29 @@ int launch_skinny(const Matrix& x, const Matrix& w0, const Matrix* w1, const Mat
   p.kept = kept;
   p.kept_stride = kept_stride;
   p.stage_bytes = (Gated ? 2 : 1) * kOperandBytes + p.width * kStep * 2;
-  p.stages = (220 * 1024) / p.stage_bytes;
+  // Two blocks fit on an SM, so that clusters of any size find places for as many tiles as there are (one block an SM with twice the
+  // stages: 15 clusters of 8 run at one time, and the sixteenth tile of a product with 2048 outputs took as long as the other fifteen;
+  // one token, 2048 x 5632: 27.5 us against 21.9), as long as each has three stages; with more tokens a block has the SM to itself
+  // (64 tokens: 31.8 us with two stages each). As many blocks a tile as there are places for, each with two steps of the
+  // reduction at least.
+  const int per_sm = 3 * p.stage_bytes <= 110 * 1024 ? 2 : 1;
+  const size_t sums = (size_t)(Gated ? 2 : 1) * p.width * kBlockRows * 4;
+  p.stages = (per_sm == 2 ? 110 : 220) * 1024 / p.stage_bytes;
   if (p.stages > 8) p.stages = 8;
-  size_t smem = (size_t)p.stages * p.stage_bytes + 1024;
-  const size_t sums = (size_t)(Gated ? 2 : 1) * p.width * kBlockRows * 4 + 1024;
-  if (smem < sums) smem = sums;
-  // as many blocks a tile as it takes to give every SM one, each with two stages of the reduction at least
+  size_t smem = (size_t)p.stages * p.stage_bytes;
+  smem = (smem > sums ? smem : sums) + 1024;
+  auto places = [per_sm](int cl) {
+    static ClusterMemo known[2];
+    return active_clusters(known[per_sm - 1], reinterpret_cast<const void*>(skinny_kernel<T, Gated>), kSkinnyThreads,
+                           (per_sm == 2 ? 111 : 221) * 1024, per_sm, cl);
+  };
   const int tiles = tiles_of(w0.rows, kBlockRows);
-  int split = device_sm_count() / tiles;
-  if (split > kMaxSplit) split = kMaxSplit;
-  if (split > p.steps / 2) split = p.steps / 2;
-  if (split < 1) split = 1;
+  int split = kMaxSplit;
+  while (split > 1 && (split > p.steps / 2 || tiles > places(split))) --split;
   uint32_t* status = device_status_word();
   if (!status) return record_cuda_error(cudaGetLastError());
   auto kernel = skinny_kernel<T, Gated>;
-  GDN2_CUDA_TRY(ensure_dynamic_smem(reinterpret_cast<const void*>(kernel), 224 * 1024));
+  GDN2_CUDA_TRY(ensure_dynamic_smem(reinterpret_cast<const void*>(kernel), smem));
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = 1;

@@ -25,8 +25,8 @@
 // training step leaves the state that enters every 64th token ("marks", 1/16 byte a channel and token) and the backward pass
 // composes the 64 tokens of its tile again from there.
 #include <algorithm>
-#include <atomic>
 
+#include "clusters.cuh"
 #include "common.cuh"
 #include "tc_utils.cuh"
 #include "tensor_map.cuh"
@@ -565,35 +565,11 @@ __global__ void __launch_bounds__(128) scan_steps_kernel(const __grid_constant__
 
 // ---------------------------------------------------------------- launches
 
-// Clusters of cl blocks that run at one time when per_sm blocks fit on an SM: a cluster lies within a group of SMs, and what does
-// not fill one up is lost (B200, one block an SM: 148, 74, 45, 33, 26, 22, 15 and 15 clusters of 1 to 8). Asked once per device.
-int active_clusters(int per_sm, int cl) {
-  static std::atomic<int> known[64][3][kMaxCluster];
-  int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) dev = 63;
-  std::atomic<int>& k = known[dev][per_sm - 1][cl - 1];
-  int n = k.load();
-  if (n > 0) return n;
-  auto kernel = scan_forward_kernel<__nv_bfloat16, 8, false, false, true>;
-  const size_t smem = (size_t)228 * 1024 / per_sm - 1024 - sizeof(Shared<8, false>) - 512;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = cl;
-  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(cl);
-  cfg.blockDim = dim3(8 * 32);
-  cfg.dynamicSmemBytes = smem;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  if (ensure_dynamic_smem(reinterpret_cast<const void*>(kernel), smem) != cudaSuccess ||
-      cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess || n <= 0) {
-    cudaGetLastError();                                // not this call's failure: fall back on an estimate
-    n = per_sm * device_sm_count() / cl;
-    return n > 0 ? n : 1;
-  }
-  k.store(n);
-  return n;
+// Clusters of cl blocks that run at one time when per_sm blocks fit on an SM
+int places(int per_sm, int cl) {
+  static ClusterMemo known[3];
+  const void* kernel = reinterpret_cast<const void*>(scan_forward_kernel<__nv_bfloat16, 8, false, false, true>);
+  return active_clusters(known[per_sm - 1], kernel, 8 * 32, (size_t)228 * 1024 / per_sm - 1024 - sizeof(Shared<8, false>) - 512, per_sm, cl);
 }
 
 // How a scan is laid out: warps of a block, blocks of a cluster, stages of a block's feed: the quickest by this account of it. A
@@ -621,7 +597,7 @@ Layout layout(int64_t rows, int64_t longest, double average, size_t token_bytes,
       for (int per_sm = W > 8 ? 1 : back ? 2 : 3; per_sm >= 1; --per_sm) {     // the kernels' launch bounds, or fewer blocks and more stages
         const size_t room = (size_t)228 * 1024 / per_sm - 1024 - fixed - slots;
         if (room < 2 * stage) continue;
-        const int64_t most = active_clusters(per_sm, cl);
+        const int64_t most = places(per_sm, cl);
         const double chain = (back ? (W > 8 ? 2.8 : 1.85) : (W > 8 ? 1.45 : 0.95)) + (cl > 1 ? 0.2 + 0.02 * cl : 0.0) + (fed ? 0.0 : 1.2);
         const int64_t rounds = (tiles + cl - 1) / cl;
         double cost;

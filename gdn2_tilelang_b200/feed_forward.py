@@ -77,7 +77,7 @@ def gated_feed_forward(x, w_gate, w_up, w_down, activation="silu"):
         if call is not None and not K.checks_status:       # the call in one native function, gradient included
             res = call(x, w_gate, w_up, w_down, _cabi.ACTIVATIONS[activation])
             if res is not None:
-                K.launches += res[1]
+                K._launches += res[1]
                 return res[0]
     _check(x, w_gate, w_up, w_down, activation)
     out_shape = (*x.shape[:-1], w_down.shape[0])

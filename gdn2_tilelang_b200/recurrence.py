@@ -82,7 +82,7 @@ def _plain(v, g, w, state, want_final, in_place=False, offsets=()):
     res = call(v, g, w, state, want_final, in_place, offsets)
     if res is None:
         return None
-    K.launches += res[2]
+    K._launches += res[2]
     return res[0], res[1]
 
 
