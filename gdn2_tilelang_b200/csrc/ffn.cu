@@ -59,6 +59,7 @@ struct Problem {
   int tiles_m, tiles_n;
   int split_m;                  // > 0: tiles from this one on take a[1] and out[1], their rows counted from there (dWg, dWu)
   int M, N;                     // rows and columns of the result (of one part)
+  int split;                    // kPlain: pairs of a cluster that share a tile's reduction; > 1: a cluster a tile
   int save;                     // kGated: a and u are kept; kGatedBackward: h is wanted
   void* plain_out[2];           // results whose rows do not start on 16 bytes are stored by threads
   int64_t out_stride;
@@ -112,10 +113,10 @@ __device__ __forceinline__ void mma_pair(uint32_t d, uint64_t a, uint64_t b, uin
                "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}"
                ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
 }
-// arrives on the barrier at this offset of both blocks once every product issued so far has completed
-__device__ __forceinline__ void commit_pair(uint64_t* bar) {
+// arrives on the barrier at this offset of both blocks of a pair once every product issued so far has completed
+__device__ __forceinline__ void commit_pair(uint64_t* bar, uint32_t leader) {
   asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
-               ::"r"(tc::smem_u32(bar)), "h"((uint16_t)3) : "memory");
+               ::"r"(tc::smem_u32(bar)), "h"((uint16_t)(3u << leader)) : "memory");
 }
 __device__ __forceinline__ void arrive_remote(uint32_t bar) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
@@ -291,8 +292,88 @@ __device__ __forceinline__ void tile_at(const Problem& p, int i, int& m, int& n)
   n = (i - b * per) / rows;
 }
 
+// The pairs of a cluster have each summed a part of one tile's reduction: each finishes 256 / split of its columns. What it has of the
+// others' columns goes to their shared memory (the ring: every product has read it, in every block of the cluster), and the
+// parts are added in their order. By all threads of all blocks of the cluster.
+template <typename T>
+__device__ __forceinline__ void join_parts(const Maps& maps, const Problem& p, Shared& sh, char* ring, char* staging, uint32_t tmem, int tile,
+                                           int rank, int part, int split, uint32_t* status) {
+  const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5, quad = wid & 3, half = (wid - 4) >> 2;
+  const int own = kTile / split, mine = own / 2;         // a pair's columns, a warp's
+  bool ok = false;
+  if (wid >= 4) {
+    ok = tc::mbar_wait_warp(&sh.done[0], 0, &sh.abort, status, kWaitCode);
+    tc::tc_fence_after_sync();
+  }
+  __syncthreads();
+  cluster_sync();
+  const uint32_t acc = tmem + ((uint32_t)(quad * 32) << 16);
+  const uint32_t parts = tc::smem_u32(ring) + (quad * 32 + lane) * 16;      // [part][column / 4][row][4]
+  if (ok)
+    for (int o = 0; o < split; ++o) {
+      if (o == part) continue;
+      const uint32_t to = in_block(parts + (part < o ? part : part - 1) * own * kBlockRows * 4, 2 * o + rank);
+      for (int c = half * mine; c < (half + 1) * mine; c += 32) {
+        float x[32];
+        tc::tmem_ld32(acc + o * own + c, x);
+        tc::tmem_ld_wait();
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(to + (c / 4 + j) * kBlockRows * 16), "f"(x[4 * j]),
+                       "f"(x[4 * j + 1]), "f"(x[4 * j + 2]), "f"(x[4 * j + 3]) : "memory");
+      }
+    }
+  __syncthreads();
+  cluster_sync();
+  if (ok) {
+    int m, n;
+    tile_at(p, tile, m, n);
+    const bool lower = p.split_m > 0 && m >= p.split_m;
+    const int row = (lower ? m - p.split_m : m) * kTile + rank * kBlockRows + quad * 32;
+    char* piece = staging + (wid - 4) * kChunkBytes;
+    T* plain = static_cast<T*>(p.plain_out[lower]);
+    for (int c = half * mine; c < (half + 1) * mine; c += 32) {
+      float x[32], sum[32] = {};
+      tc::tmem_ld32(acc + part * own + c, x);
+      tc::tmem_ld_wait();
+      for (int q = 0; q < split; ++q) {
+        const uint32_t from = parts + (q < part ? q : q - 1) * own * kBlockRows * 4;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          float4 f = make_float4(x[4 * j], x[4 * j + 1], x[4 * j + 2], x[4 * j + 3]);
+          if (q != part)
+            asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(f.x), "=f"(f.y), "=f"(f.z), "=f"(f.w)
+                         : "r"(from + (c / 4 + j) * kBlockRows * 16) : "memory");
+          sum[4 * j] += f.x; sum[4 * j + 1] += f.y; sum[4 * j + 2] += f.z; sum[4 * j + 3] += f.w;
+        }
+      }
+      const int col = n * kTile + part * own + c;
+      chunk_free(lane);
+      put_row64<T>(piece, lane, sum);
+      if (row >= p.M || col >= p.N) continue;
+      if (plain == nullptr) {
+        tc::fence_async_smem();
+        __syncwarp();
+        if (lane == 0) {
+          tma_store(&maps.out[lower], col, row, tc::smem_u32(piece));
+          tc::bulk_commit();
+        }
+      } else {
+        __syncwarp();
+        for (int r = 0; r < 32 && row + r < p.M; ++r)
+          if (col + lane < p.N)
+            plain[(int64_t)(row + r) * p.out_stride + col + lane] = *reinterpret_cast<const T*>(piece + row64_at(r, lane >> 3) + (lane & 7) * 2);
+        __syncwarp();
+      }
+    }
+    if (lane == 0) tc::bulk_wait_all();
+    __syncwarp();
+  }
+  tc::tc_fence_before_sync();
+}
+
 template <typename T, int K, bool A_MN, bool B_MN, bool Gelu>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__(kThreads, 1)
 product_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Problem p, uint32_t* status) {
   constexpr int S = stages<K>();
   extern __shared__ __align__(1024) char smem_raw[];
@@ -300,9 +381,11 @@ product_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Proble
   char* ring = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   char* staging = ring + S * kStageBytes;
   const int tid = threadIdx.x, lane = tid & 31, wid = tid >> 5;
-  const uint32_t rank = cluster_rank();
-  const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+  const uint32_t block = cluster_rank(), rank = block & 1, leader = block & ~1u;
+  const int split = K == kPlain ? p.split : 1, part = (int)block >> 1;      // pairs of the cluster, and which this is
+  const int pair = blockIdx.x / (2 * split), pairs = gridDim.x / (2 * split);
   const int tiles = p.tiles_m * p.tiles_n, steps = p.steps[0] + p.steps[1];
+  const int first = steps * part / split, behind = steps * (part + 1) / split;      // this pair's share of the reduction
 
   if (wid == 0 && lane == 0) {
     for (int i = 0; i < S; ++i) {
@@ -338,12 +421,12 @@ product_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Proble
         const bool lower = p.split_m > 0 && m >= p.split_m;
         const int row_a = (lower ? m - p.split_m : m) * kTile + rank * kBlockRows;
         const int row_b = K == kGated ? n * kBlockRows : n * kTile + (int)rank * kBlockRows;
-        for (int k = 0; k < steps; ++k) {
+        for (int k = first; k < behind; ++k) {
           const int run = k >= p.steps[0], at = (run ? k - p.steps[0] : k) * kStep;
           const CUtensorMap* ma = &maps.a[lower || run ? 1 : 0];
           const CUtensorMap* mb = &maps.b[K == kGated ? (int)rank : run];
           if (!tc::mbar_wait(&sh.empty[s], phase ^ 1, &sh.abort, status, kWaitCode)) { ok = false; break; }
-          const uint32_t bar = in_block(tc::smem_u32(&sh.full[s]), 0), dst = tc::smem_u32(ring + s * kStageBytes);
+          const uint32_t bar = in_block(tc::smem_u32(&sh.full[s]), leader), dst = tc::smem_u32(ring + s * kStageBytes);
           if (rank == 0) tc::mbar_expect_tx(&sh.full[s], 2 * kStageBytes);
           if constexpr (A_MN) {
             tma_load_pair(dst, ma, row_a, at, bar);
@@ -372,18 +455,18 @@ product_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Proble
         if (!tc::mbar_wait(&sh.taken[buf], taken, &sh.abort, status, kWaitCode)) break;
         tc::tc_fence_after_sync();
         const uint32_t d = tmem + buf * kTile;
-        for (int k = 0; k < steps; ++k) {
+        for (int k = first; k < behind; ++k) {
           if (!tc::mbar_wait(&sh.full[s], phase, &sh.abort, status, kWaitCode)) { ok = false; break; }
           tc::tc_fence_after_sync();
           const uint32_t at = tc::smem_u32(ring + s * kStageBytes);
           uint64_t a = operand_desc<A_MN>(at), b = operand_desc<B_MN>(at + kOperandBytes);
 #pragma unroll
           for (int q = 0; q < kStep / 16; ++q)
-            mma_pair(d, a + q * operand_step<A_MN>(), b + q * operand_step<B_MN>(), idesc, (k | q) != 0);
-          commit_pair(&sh.empty[s]);
+            mma_pair(d, a + q * operand_step<A_MN>(), b + q * operand_step<B_MN>(), idesc, k > first || q > 0);
+          commit_pair(&sh.empty[s], leader);
           if (++s == S) { s = 0; phase ^= 1; }
         }
-        if (ok) commit_pair(&sh.done[buf]);
+        if (ok) commit_pair(&sh.done[buf], leader);
         if (buf == 1) taken ^= 1;
         buf ^= 1;
       }
@@ -394,7 +477,7 @@ product_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Proble
     const int quad = wid & 3, half = (wid - 4) >> 2, ew = wid - 4;
     char* chunk = staging + ew * (staging_bytes<K>() / kEpiWarps);
     const uint32_t lanes = (uint32_t)(quad * 32) << 16;
-    const uint32_t taken0 = in_block(tc::smem_u32(&sh.taken[0]), 0), taken1 = in_block(tc::smem_u32(&sh.taken[1]), 0);
+    const uint32_t taken0 = in_block(tc::smem_u32(&sh.taken[0]), leader), taken1 = in_block(tc::smem_u32(&sh.taken[1]), leader);
     int buf = 0, phase = 0;
     int loads = 0;                                    // kGatedBackward: pieces loaded so far
     auto load_piece = [&](int i, int c) {             // 32 columns of a and u, piece c of this warp's half of tile i
@@ -412,7 +495,7 @@ product_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Proble
       }
     };
     if constexpr (K == kGatedBackward) load_piece(pair, 0);
-    for (int i = pair; i < tiles; i += pairs) {
+    for (int i = pair; split == 1 && i < tiles; i += pairs) {
       int m, n;
       tile_at(p, i, m, n);
       const bool lower = p.split_m > 0 && m >= p.split_m;
@@ -530,6 +613,8 @@ product_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Proble
     if (lane == 0) tc::bulk_wait_all();               // nothing reads this block's memory any more
     __syncwarp();
   }
+  if constexpr (K == kPlain)
+    if (split > 1) join_parts<T>(maps, p, sh, ring, staging, tmem, pair, (int)rank, part, split, status);
   __syncthreads();
   after_a_failure(&sh.abort);
   cluster_sync();                                     // neither block leaves while the other's products or copies need it
@@ -541,7 +626,8 @@ product_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Proble
 
 constexpr int kSkinnyThreads = 256;
 constexpr int kMaxSplit = 8;
-constexpr int kSkinnyTokens = 64;                // the most tokens of a call that goes this way
+constexpr int kSkinnyTokens = 128;               // the most tokens of a call that goes this way
+constexpr int kSkinnyColumns = 2 * kSkinnyTokens; // of tensor memory: the gate's sums, the up projection's
 
 struct __align__(64) SkinnyMaps {
   CUtensorMap w[2], x;                           // weights (Wg, Wu; or Wd alone) in boxes of 128 rows, tokens in boxes of `width`
@@ -588,7 +674,7 @@ __global__ void __launch_bounds__(kSkinnyThreads, 2) skinny_kernel(const __grid_
     tc::fence_async_smem();
     for (int i = 0; i < first; ++i) fetch(k0 + i, i);
   }
-  if (wid == 2) tc::tmem_alloc(&sh.tmem, 128);
+  if (wid == 2) tc::tmem_alloc(&sh.tmem, kSkinnyColumns);
   tc::tc_fence_before_sync();
   __syncthreads();
   tc::tc_fence_after_sync();
@@ -619,7 +705,7 @@ __global__ void __launch_bounds__(kSkinnyThreads, 2) skinny_kernel(const __grid_
           const uint32_t acc = k > k0 || q > 0;
           tc::mma_bf16(tmem, w + q * operand_step<false>(), x + q * operand_step<false>(), idesc, acc);
           if constexpr (Gated)
-            tc::mma_bf16(tmem + 64, w + (kOperandBytes >> 4) + q * operand_step<false>(), x + q * operand_step<false>(), idesc, acc);
+            tc::mma_bf16(tmem + kSkinnyTokens, w + (kOperandBytes >> 4) + q * operand_step<false>(), x + q * operand_step<false>(), idesc, acc);
         }
         tc::mma_commit(&sh.empty[s]);
         if (++s == p.stages) { s = 0; phase ^= 1; }
@@ -637,7 +723,7 @@ __global__ void __launch_bounds__(kSkinnyThreads, 2) skinny_kernel(const __grid_
 #pragma unroll
         for (int g = 0; g < (Gated ? 2 : 1); ++g) {
           float x[16];
-          tc::tmem_ld16(tmem + ((uint32_t)(quad * 32) << 16) + g * 64 + n, x);
+          tc::tmem_ld16(tmem + ((uint32_t)(quad * 32) << 16) + g * kSkinnyTokens + n, x);
           tc::tmem_ld_wait();
 #pragma unroll
           for (int j = 0; j < 16; ++j) part[(g * p.width + n + j) * kBlockRows + quad * 32 + lane] = x[j];
@@ -702,7 +788,7 @@ __global__ void __launch_bounds__(kSkinnyThreads, 2) skinny_kernel(const __grid_
   }
   __syncthreads();
   if (CL > 1) cluster_sync();                         // no block leaves while another reads its sums
-  if (wid == 2) tc::tmem_dealloc(tmem, 128);
+  if (wid == 2) tc::tmem_dealloc(tmem, kSkinnyColumns);
 }
 
 // ---------------------------------------------------------------- rows to a pitch of 16 bytes
@@ -769,10 +855,39 @@ int launch_product(const Maps& maps, const Problem& p, cudaStream_t st) {
   if (!status) return record_cuda_error(cudaGetLastError());
   auto kernel = product_kernel<T, K, A_MN, B_MN, Gelu>;
   GDN2_CUDA_TRY(ensure_dynamic_smem(reinterpret_cast<const void*>(kernel), smem_bytes<K>()));
-  const int tiles = p.tiles_m * p.tiles_n, pairs = device_sm_count() / 2;
-  kernel<<<2 * (tiles < pairs ? tiles : pairs), kThreads, smem_bytes<K>(), st>>>(maps, p, status);
-  GDN2_CUDA_TRY(cudaGetLastError());
+  const int tiles = p.tiles_m * p.tiles_n, pairs = device_sm_count() / 2, split = K == kPlain ? p.split : 1;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 2 * split;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(2 * split * (split > 1 || tiles < pairs ? tiles : pairs));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = smem_bytes<K>();
+  cfg.stream = st;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  GDN2_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, maps, p, status));
   return GDN2_OK;
+}
+
+// Pairs that share a tile's reduction: with few tiles and a long reduction most SMs would idle. A step is 0.27 us of a pair, joining
+// the parts 3 us; clusters of 4 and 8 blocks find places for 33 and 15 tiles.
+template <typename T, bool A_MN, bool B_MN> int split_of(int tiles, int steps) {
+  static ClusterMemo known;
+  int best = 1;
+  double least = steps * 0.27;
+  for (int s = 2; s <= 4; s *= 2) {
+    if (steps < 2 * s || tiles > active_clusters(known, reinterpret_cast<const void*>(product_kernel<T, kPlain, A_MN, B_MN, false>), kThreads,
+                                                 smem_bytes<kPlain>(), 1, 2 * s))
+      continue;
+    const double cost = steps * 0.27 / s + 3.0;
+    if (cost < least) {
+      best = s;
+      least = cost;
+    }
+  }
+  return best;
 }
 
 #define GDN2_MAP(m, matrix, box)                                     \
@@ -822,8 +937,8 @@ int gated_backward(const Matrix& dy, const Matrix& wd, void* kept, const Matrix&
 
 int set_out(Maps& maps, Problem& p, int part, const Matrix& out, int dtype) {
   p.out_stride = out.stride;
-  if (aligned_rows(out)) GDN2_MAP(maps.out[part], out, 32);
-  else p.plain_out[part] = const_cast<void*>(out.p);
+  if (!aligned_rows(out)) p.plain_out[part] = const_cast<void*>(out.p);
+  else if (!make_map(&maps.out[part], out, 32, dtype, p.split > 1 ? 32 : 64)) return GDN2_ERR_UNSUPPORTED;
   return GDN2_OK;
 }
 
@@ -837,10 +952,11 @@ int product(const Matrix* a, const Matrix* b, int runs, const Matrix& out, int d
     GDN2_MAP(maps.b[i], b[i], B_MN ? kStep : kBlockRows);
     p.steps[i] = steps_of(A_MN ? a[i].rows : a[i].cols);
   }
-  const int rc = set_out(maps, p, 0, out, dtype);
-  if (rc != GDN2_OK) return rc;
   p.tiles_m = tiles_of(out.rows, kTile);
   p.tiles_n = tiles_of(out.cols, kTile);
+  p.split = split_of<T, A_MN, B_MN>(p.tiles_m * p.tiles_n, p.steps[0] + p.steps[1]);
+  const int rc = set_out(maps, p, 0, out, dtype);
+  if (rc != GDN2_OK) return rc;
   p.M = (int)out.rows;
   p.N = (int)out.cols;
   return launch_product<T, kPlain, A_MN, B_MN>(maps, p, st);
@@ -853,13 +969,14 @@ int two_weight_gradients(const Matrix& a0, const Matrix& a1, const Matrix& b, co
   GDN2_MAP(maps.a[0], a0, kStep);
   GDN2_MAP(maps.a[1], a1, kStep);
   GDN2_MAP(maps.b[0], b, kStep);
-  int rc = set_out(maps, p, 0, out0, dtype);
-  if (rc == GDN2_OK) rc = set_out(maps, p, 1, out1, dtype);
-  if (rc != GDN2_OK) return rc;
   p.steps[0] = steps_of(b.rows);
   p.split_m = tiles_of(out0.rows, kTile);
   p.tiles_m = 2 * p.split_m;
   p.tiles_n = tiles_of(out0.cols, kTile);
+  p.split = split_of<T, true, true>(p.tiles_m * p.tiles_n, p.steps[0]);
+  int rc = set_out(maps, p, 0, out0, dtype);
+  if (rc == GDN2_OK) rc = set_out(maps, p, 1, out1, dtype);
+  if (rc != GDN2_OK) return rc;
   p.M = (int)out0.rows;
   p.N = (int)out0.cols;
   return launch_product<T, kPlain, true, true>(maps, p, st);
