@@ -800,18 +800,29 @@ struct Copies {
   int64_t rows[kMaxCopies], src_stride[kMaxCopies], dst_stride[kMaxCopies];
   int cols[kMaxCopies];
 };
-// 8 elements a thread; what lies behind a row's end is zero
+// 8 elements a thread, read as the 4-byte words that hold them (a row may start in the middle of one) and shifted into place; what
+// lies behind a row's end is zero, and words behind it are not read. Element by element it was bound by its loads: 9.5 us instead of
+// 6.5 for the four operands of 1003 x 1001 x 2731.
 __global__ void __launch_bounds__(256) align_rows_kernel(const __grid_constant__ Copies c) {
-  const int j = blockIdx.y, per = (c.cols[j] + 7) / 8;
+  const int j = blockIdx.y, cols = c.cols[j], per = (cols + 7) / 8;
   const int64_t n = c.rows[j] * per;
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
     const int64_t r = i / per;
-    const int at = (int)(i - r * per) * 8;
+    const int at = (int)(i - r * per) * 8, left = min(cols - at, 8);          // elements of this piece
     const uint16_t* s = c.src[j] + r * c.src_stride[j] + at;
-    uint16_t e[8];
+    const int odd = (int)(reinterpret_cast<uintptr_t>(s) >> 1) & 1;
+    const uint32_t* word = reinterpret_cast<const uint32_t*>(s - odd);
+    const int words = (left + odd + 1) / 2;
+    uint32_t w[5], e[4];
 #pragma unroll
-    for (int q = 0; q < 8; ++q) e[q] = at + q < c.cols[j] ? s[q] : (uint16_t)0;
-    *reinterpret_cast<uint4*>(c.dst[j] + r * c.dst_stride[j] + at) = *reinterpret_cast<const uint4*>(e);
+    for (int q = 0; q < 5; ++q) w[q] = q < words ? __ldg(word + q) : 0u;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      e[q] = odd ? __funnelshift_r(w[q], w[q + 1], 16) : w[q];
+      if (2 * q >= left) e[q] = 0u;
+      else if (2 * q + 1 >= left) e[q] &= 0xffffu;
+    }
+    *reinterpret_cast<uint4*>(c.dst[j] + r * c.dst_stride[j] + at) = make_uint4(e[0], e[1], e[2], e[3]);
   }
 }
 
