@@ -266,6 +266,7 @@ __global__ void __launch_bounds__(W * 32, W == 8 ? 3 : 1) scan_forward_kernel(co
   T* o = static_cast<T*>(a.o) + (p.batch * a.S + p.start) * a.D;
   float2 carry = make_float2(0.f, 0.f);               // the exchanging warp's: the last, whose run ends the tile
   if (wid == W - 1 && a.first) carry = ch.load(a.first + (int64_t)p.seq * a.D);
+  if (wid == W - 1) sh.entering[lane] = carry;        // loaded before the first run is sent: the state may be updated in place by another block
 
   const int64_t tiles = (p.len + kTile - 1) / kTile, rounds = (tiles + p.CL - 1) / p.CL;
   auto fetch = [&](int64_t it, int s) {               // by one thread
@@ -362,6 +363,7 @@ __global__ void __launch_bounds__(W * 32, W == 8 ? 2 : 1) scan_backward_kernel(c
   const int64_t out0 = (p.batch * a.S + p.start) * a.D;
   float2 carry = make_float2(0.f, 0.f);               // the exchanging warp's: the first, whose run ends the tile from behind
   if (wid == 0 && a.first) carry = ch.load(a.first + (int64_t)p.seq * a.D);
+  if (wid == 0) sh.entering[lane] = carry;            // loaded before the first run is sent, as in the forward pass
 
   const int64_t tiles = (p.len + kTile - 1) / kTile, rounds = (tiles + p.CL - 1) / p.CL;
   auto fetch = [&](int64_t it, int s) {
@@ -678,6 +680,15 @@ int launch_scan(const Args& a0, const Tables& tb, int64_t longest, double averag
   return GDN2_OK;
 }
 
+// Rows that no tensor map can describe are loaded by the threads
+template <typename T, bool Gate, bool Packed, bool Fed>
+int launch_any(const Args& a, const Tables& tb, int64_t longest, double average, bool backward, cudaStream_t st) {
+  const int rc = launch_scan<T, Gate, Packed, Fed>(a, tb, longest, average, backward, st);
+  if constexpr (Fed)
+    if (rc == GDN2_ERR_UNSUPPORTED) return launch_scan<T, Gate, Packed, false>(a, tb, longest, average, backward, st);
+  return rc;
+}
+
 template <typename T, int VEC, bool Gate>
 int launch_all(const Args& a, const int64_t* cu, bool backward, cudaStream_t st) {
   if (!cu) {
@@ -690,7 +701,7 @@ int launch_all(const Args& a, const int64_t* cu, bool backward, cudaStream_t st)
       GDN2_CUDA_TRY(cudaGetLastError());
       return GDN2_OK;
     }
-    return launch_scan<T, Gate, false, (VEC > 1)>(a, none, a.S, (double)a.S, backward, st);
+    return launch_any<T, Gate, false, (VEC > 1)>(a, none, a.S, (double)a.S, backward, st);
   }
   int64_t mark = 0;
   for (int i0 = 0; i0 < a.sequences; i0 += kMaxPacked) {
@@ -717,7 +728,7 @@ int launch_all(const Args& a, const int64_t* cu, bool backward, cudaStream_t st)
     part.sequences = tb.n;
     if (a.first) part.first = a.first + (int64_t)i0 * a.D;
     if (a.last) part.last = a.last + (int64_t)i0 * a.D;
-    const int rc = launch_scan<T, Gate, true, (VEC > 1)>(part, tb, longest, average, backward, st);
+    const int rc = launch_any<T, Gate, true, (VEC > 1)>(part, tb, longest, average, backward, st);
     if (rc != GDN2_OK) return rc;
   }
   return GDN2_OK;

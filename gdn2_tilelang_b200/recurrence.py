@@ -102,6 +102,10 @@ def gated_recurrence(v, g, w=None, initial_state=None, output_final_state=False,
     A backward pass that is captured into a CUDA graph follows PyTorch's rule for it: no other graph of the same leaves alive
     on another stream (``torch.autograd.grad`` on inputs made for the capture is safe).
     """
+    if g.is_floating_point():                          # (float() of a float32 tensor is the tensor)
+        g = g.float()
+    if initial_state is not None and initial_state.is_floating_point():
+        initial_state = initial_state.float()
     if cu_seqlens is None and v.is_cuda:
         res = _plain(v, g, w, initial_state, output_final_state)
         if res is not None:
@@ -117,8 +121,6 @@ def gated_recurrence(v, g, w=None, initial_state=None, output_final_state=False,
         if not initial_state.is_floating_point():
             raise TypeError(f"initial_state must be a floating-point tensor, got {initial_state.dtype}")
         _check_devices(v, initial_state)
-        initial_state = initial_state.float()
-    g = g.float()
     if offsets is not None:
         res = _plain(v, g, w, initial_state, output_final_state, offsets=offsets)
         if res is not None:
@@ -140,6 +142,8 @@ def gated_recurrence_decode(v, g, w, state):
     """Decode ``n`` tokens (``[B, n, ...]``), updating ``state [B, ...]`` (float32, contiguous) in place. ``w`` may be ``None``.
 
     Returns ``o [B, n, ...]`` in ``v.dtype``. No gradient."""
+    if g.is_floating_point():
+        g = g.float()
     if v.is_cuda:
         res = _plain(v, g, w, state, True, in_place=True)
         if res is not None:
@@ -156,7 +160,7 @@ def gated_recurrence_decode(v, g, w, state):
     if v.numel() == 0:
         return torch.empty_like(v, memory_format=torch.contiguous_format)
     K = _cabi.kernels()
-    rows = [None if t is None else t.flatten(2) for t in (v, g.float(), w)]
+    rows = [None if t is None else t.flatten(2) for t in (v, g, w)]
     o, _, _ = K.recurrence(*rows, state.view(B, -1), None, in_place=True)
     K.maybe_check_device_status(v.device)
     return o.view(v.shape)

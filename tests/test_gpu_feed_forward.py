@@ -272,3 +272,33 @@ def test_launches_are_counted():
     y = gdn2.gated_feed_forward(x, wg.requires_grad_(), wu, wd)
     y.backward(dy)
     assert K.launches == before + 2 + 2 + 2            # the gated gradient and the pair of weight gradients
+
+
+def test_offsets_beyond_32_bits():
+    """Inner activations of more than 2^31 elements: the last rows against the same tokens alone."""
+    T, hid, inn = 400_000, 64, 5632
+    x, wg, wu, wd, _ = make(T, hid, inn, BF)
+    assert T * inn > 1 << 31
+    y = gdn2.gated_feed_forward(x, wg, wu, wd)
+    for rows in (slice(0, 300), slice(T - 300, T)):
+        orc.assert_within(y[rows], *orc.evaluate(x[rows], wg, wu, wd, "silu")["y"], "y")
+    leaf = x.clone().requires_grad_()
+    dx = torch.autograd.grad(gdn2.gated_feed_forward(leaf, wg, wu, wd), leaf, torch.ones_like(x))[0]
+    for rows in (slice(0, 300), slice(T - 300, T)):
+        want = orc.evaluate(x[rows], wg, wu, wd, "silu", torch.ones_like(x[rows]))
+        orc.assert_within(dx[rows], *want["dx"], "dx")
+
+
+@pytest.mark.parametrize("T", [5, 300])
+def test_two_streams_at_once(T):
+    x, wg, wu, wd, _ = make(T, 512, 1536, BF)
+    want = gdn2.gated_feed_forward(x, wg, wu, wd)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    outs = []
+    for _ in range(20):
+        for st in streams:
+            with torch.cuda.stream(st):
+                outs.append(gdn2.gated_feed_forward(x, wg, wu, wd))
+    torch.cuda.synchronize()
+    assert all(torch.equal(y, want) for y in outs)

@@ -341,3 +341,53 @@ def test_launches_are_counted():
     assert K.launches == before + 1
     o.sum().backward()
     assert K.launches == before + 2
+
+
+def test_offsets_beyond_32_bits():
+    """More than 2^31 elements an input. Memory is 20 tokens here: the last rows from zero, 3000 tokens before them, to 32 bits."""
+    S, D = (1 << 21) + 77, 1032
+    gen = torch.Generator(device="cuda").manual_seed(0)
+    v = torch.empty(1, S, D, dtype=BF, device="cuda").normal_(generator=gen)
+    g = torch.full((1, S, D), -0.05, device="cuda")
+    assert v.numel() > 1 << 31
+    o, fin = gdn2.gated_recurrence(v, g, output_final_state=True)
+    lo = S - 4000
+    tail, tfin = gdn2.gated_recurrence(v[:, lo:], g[:, lo:], output_final_state=True)
+    # 3000 tokens of exp(-0.05) leave e^-150 of what came before: the same sums but for the order they are composed in
+    mag = orc.STEP * 20 * 20 * 5                                   # 8 u a step, a memory and a magnitude of 20 and |v| < 5
+    assert float((fin - tfin).abs().max()) <= 2 * mag
+    assert float((o[:, lo + 3000:].float() - tail[:, 3000:].float()).abs().max()) <= 2 * mag + 2**-8 * 20
+    del o, tail
+    do = torch.ones(1, 1, 1, dtype=BF, device="cuda").expand(1, S, D)
+    leaf = v.requires_grad_()
+    out, _ = gdn2.gated_recurrence(leaf, g)
+    dv = torch.autograd.grad(out, leaf, do)[0]
+    a = float(torch.tensor(-0.05, dtype=torch.float64).exp())
+    assert torch.all(dv[0, -1] == 1) and torch.all(dv[0, 0] == dv[0, 5000]) and abs(float(dv[0, 0, 0]) - 1 / (1 - a)) <= 2**-8 / (1 - a)
+
+
+def test_two_streams_at_once():
+    v, g, w, s = on_gpu(*make(2, 3000, 512, BF))
+    want = gdn2.gated_recurrence(v, g, w, s, True)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    outs = []
+    for _ in range(20):
+        for st in streams:
+            with torch.cuda.stream(st):
+                outs.append(gdn2.gated_recurrence(v, g, w, s, True))
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, want[0]) and torch.equal(f, want[1]) for o, f in outs)
+
+
+def test_other_types_of_decay_and_state():
+    v, g, w, s = make(2, 40, 64, BF)
+    g, s = g.to(BF), s.to(F16)
+    vc, gc, wc, sc = on_gpu(v, g, w, s, grad=True)
+    o, fin = gdn2.gated_recurrence(vc, gc, wc, sc, output_final_state=True)
+    check_forward(o, fin, orc.scan(v, g, w, s))
+    dg, ds = torch.autograd.grad(o.float().sum(), (gc, sc))
+    assert dg.dtype == BF and ds.dtype == F16
+    (_, want, _, wantds), (_, eg, _, es) = orc.gradients(v, g, w, s, torch.ones_like(v), None)
+    orc.assert_within(dg, want, eg, "dg")
+    orc.assert_within(ds, wantds, es, "dstate")
