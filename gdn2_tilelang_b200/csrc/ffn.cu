@@ -23,7 +23,9 @@
 //
 // Few tokens (skinny_kernel): the work is reading the weights once. They take the 128-row side of the product, the tokens
 // the narrow one, and the reduction of a tile is cut over the blocks of a cluster so that every SM reads; the blocks' partial
-// sums meet in distributed shared memory, added in the order of the blocks.
+// sums meet in distributed shared memory, added in the order of the blocks. The second kernel is chained to the first: it asks for its
+// first weights, which nothing before it writes, as soon as it finds a place, and for the first's results when that has completed.
+// The first is launched plainly, so everything before it is complete by then.
 #include "clusters.cuh"
 #include "common.cuh"
 #include "tc_utils.cuh"
@@ -655,13 +657,16 @@ __global__ void __launch_bounds__(kSkinnyThreads, 2) skinny_kernel(const __grid_
   const int k0 = (int)((int64_t)p.steps * rank / CL), k1 = (int)((int64_t)p.steps * (rank + 1) / CL);
   constexpr int kWeightBytes = (Gated ? 2 : 1) * kOperandBytes;
   const int token_bytes = p.width * kStep * 2;
-  auto fetch = [&](int k, int s) {
+  auto fetch_weights = [&](int k, int s) {
     const uint32_t bar = tc::smem_u32(&sh.full[s]), dst = tc::smem_u32(ring + s * p.stage_bytes);
     tc::mbar_expect_tx(&sh.full[s], kWeightBytes + token_bytes);
     tma_load(dst, &maps.w[0], k * kStep, row0, bar);
     if constexpr (Gated) tma_load(dst + kOperandBytes, &maps.w[1], k * kStep, row0, bar);
-    tma_load(dst + kWeightBytes, &maps.x, k * kStep, 0, bar);
   };
+  auto fetch_tokens = [&](int k, int s) {
+    tma_load(tc::smem_u32(ring + s * p.stage_bytes) + kWeightBytes, &maps.x, k * kStep, 0, tc::smem_u32(&sh.full[s]));
+  };
+  if constexpr (Gated) grid_launch_dependents();      // every block is in place or has been by the time this counts
   const int first = min(p.stages, k1 - k0);           // stages that are asked for before anything else
   if (wid == 0 && lane == 0) {
     for (int i = 0; i < p.stages; ++i) {
@@ -672,8 +677,11 @@ __global__ void __launch_bounds__(kSkinnyThreads, 2) skinny_kernel(const __grid_
     sh.abort = 0;
     tc::mbar_init_fence();
     tc::fence_async_smem();
-    for (int i = 0; i < first; ++i) fetch(k0 + i, i);
+    for (int i = 0; i < first; ++i) fetch_weights(k0 + i, i);
+    if constexpr (!Gated) grid_wait();                // the tokens are the gated product's results
+    for (int i = 0; i < first; ++i) fetch_tokens(k0 + i, i);
   }
+  if constexpr (!Gated) grid_wait();
   if (wid == 2) tc::tmem_alloc(&sh.tmem, kSkinnyColumns);
   tc::tc_fence_before_sync();
   __syncthreads();
@@ -685,7 +693,8 @@ __global__ void __launch_bounds__(kSkinnyThreads, 2) skinny_kernel(const __grid_
       int s = first == p.stages ? 0 : first, phase = 0;
       for (int k = k0 + first; k < k1; ++k) {
         if (!tc::mbar_wait(&sh.empty[s], phase, &sh.abort, status, kWaitCode)) break;
-        fetch(k, s);
+        fetch_weights(k, s);
+        fetch_tokens(k, s);
         if (++s == p.stages) { s = 0; phase ^= 1; }
       }
     }
@@ -1034,18 +1043,22 @@ int launch_skinny(const Matrix& x, const Matrix& w0, const Matrix* w1, const Mat
   if (!status) return record_cuda_error(cudaGetLastError());
   auto kernel = skinny_kernel<T, Gated>;
   GDN2_CUDA_TRY(ensure_dynamic_smem(reinterpret_cast<const void*>(kernel), smem));
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = 1;
   attr[0].val.clusterDim.y = split;
   attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;      // inside a capture launches stay plain (launch_chained says why)
+  const bool chained = !Gated && (cudaStreamIsCapturing(st, &capture) != cudaSuccess || capture == cudaStreamCaptureStatusNone);
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(tiles, split);
   cfg.blockDim = dim3(kSkinnyThreads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = chained ? 2 : 1;
   GDN2_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, maps, p, status));
   return GDN2_OK;
 }
