@@ -1002,6 +1002,10 @@ int two_weight_gradients(const Matrix& a0, const Matrix& a1, const Matrix& b, co
   return launch_product<T, kPlain, true, true>(maps, p, st);
 }
 
+// For the question how many clusters of two blocks an SM run at one time: of a kernel with tensor memory the runtime says one block an SM,
+// whatever it allocates
+__global__ void __launch_bounds__(kSkinnyThreads, 2) stand_in_kernel() {}
+
 template <typename T, bool Gated>
 int launch_skinny(const Matrix& x, const Matrix& w0, const Matrix* w1, const Matrix& out, void* kept, int64_t kept_stride, int gelu, int dtype,
                   cudaStream_t st) {
@@ -1024,7 +1028,8 @@ int launch_skinny(const Matrix& x, const Matrix& w0, const Matrix* w1, const Mat
   // stages: 15 clusters of 8 run at one time, and the sixteenth tile of a product with 2048 outputs took as long as the other fifteen;
   // one token, 2048 x 5632: 27.5 us against 21.9), as long as each has three stages; with more tokens a block has the SM to itself
   // (64 tokens: 31.8 us with two stages each). As many blocks a tile as there are places for, each with two steps of the
-  // reduction at least.
+  // reduction at least; over 16 tokens no more than one an SM, because every block brings the tokens, too (replayed from a graph, 24
+  // tokens 23.4 us against 23.9; one token 21.9 against 20.9 the other way).
   const int per_sm = 3 * p.stage_bytes <= 110 * 1024 ? 2 : 1;
   const size_t sums = (size_t)(Gated ? 2 : 1) * p.width * kBlockRows * 4;
   p.stages = (per_sm == 2 ? 110 : 220) * 1024 / p.stage_bytes;
@@ -1033,12 +1038,13 @@ int launch_skinny(const Matrix& x, const Matrix& w0, const Matrix* w1, const Mat
   smem = (smem > sums ? smem : sums) + 1024;
   auto places = [per_sm](int cl) {
     static ClusterMemo known[2];
-    return active_clusters(known[per_sm - 1], reinterpret_cast<const void*>(skinny_kernel<T, Gated>), kSkinnyThreads,
-                           (per_sm == 2 ? 111 : 221) * 1024, per_sm, cl);
+    return active_clusters(known[per_sm - 1], reinterpret_cast<const void*>(stand_in_kernel), kSkinnyThreads,
+                           (per_sm == 2 ? 112 : 222) * 1024, per_sm, cl);
   };
   const int tiles = tiles_of(w0.rows, kBlockRows);
   int split = kMaxSplit;
-  while (split > 1 && (split > p.steps / 2 || tiles > places(split))) --split;
+  const int blocks = p.width > 16 ? device_sm_count() : 2 * device_sm_count();
+  while (split > 1 && (split > p.steps / 2 || tiles > places(split) || tiles * split > blocks)) --split;
   uint32_t* status = device_status_word();
   if (!status) return record_cuda_error(cudaGetLastError());
   auto kernel = skinny_kernel<T, Gated>;
