@@ -242,6 +242,15 @@ __device__ __forceinline__ void get_kept(const char* upper, const char* lower, i
     }
   }
 }
+// Uses what get_kept has read, an instruction for each of its loads: loads from shared memory may wait their turn behind the warps'
+// other accesses for longer than a copy takes to arrive, so one that overwrites the piece may only be asked for when the values
+// have come back. (Without it, and with more of them waiting, an a or u in some tens of calls was the next piece's.)
+__device__ __forceinline__ void in_registers(const float (&x)[32]) {
+  uint32_t s = 0;
+#pragma unroll
+  for (int i = 0; i < 32; i += 4) s ^= __float_as_uint(x[i]);
+  asm volatile("" ::"r"(s) : "memory");
+}
 // A warp's chunk to rows row.., columns col.. of the result; what lies outside is dropped.
 template <typename T>
 __device__ __forceinline__ void store_chunk(const char* chunk, const CUtensorMap* map, T* plain, int64_t stride, int row, int col, int M,
@@ -578,6 +587,8 @@ product_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Proble
           tc::tmem_ld32(acc + half * 128 + 32 * c, d);
           get_kept(chunk, chunk + 4096, lane, a);
           get_kept(chunk + 2048, chunk + 5120, lane, u);
+          in_registers(a);
+          in_registers(u);
           __syncwarp();
           if (c < 3) load_piece(i, c + 1); else load_piece(i + pairs, 0);
           tc::tmem_ld_wait();

@@ -302,3 +302,16 @@ def test_two_streams_at_once(T):
                 outs.append(gdn2.gated_feed_forward(x, wg, wu, wd))
     torch.cuda.synchronize()
     assert all(torch.equal(y, want) for y in outs)
+
+
+@pytest.mark.parametrize("T", [40, 127, 300, 1000])
+def test_gradients_have_the_same_bits_every_time(T):
+    """Nothing is overwritten before it has been read, however the warps' loads and stores queue up."""
+    x, wg, wu, wd, dy = make(T, 256, 384, BF)
+    leaves = [t.clone().requires_grad_() for t in (x, wg, wu, wd)]
+    first = torch.autograd.grad(gdn2.gated_feed_forward(*leaves), leaves, dy)
+    differ = torch.zeros((), dtype=torch.int64, device="cuda")
+    for _ in range(300):
+        for a, b in zip(torch.autograd.grad(gdn2.gated_feed_forward(*leaves), leaves, dy), first):
+            differ += (a != b).sum()
+    assert int(differ) == 0

@@ -391,3 +391,15 @@ def test_other_types_of_decay_and_state():
     (_, want, _, wantds), (_, eg, _, es) = orc.gradients(v, g, w, s, torch.ones_like(v), None)
     orc.assert_within(dg, want, eg, "dg")
     orc.assert_within(ds, wantds, es, "dstate")
+
+
+@pytest.mark.parametrize("B,S,D", [(2, 700, 512), (1, 5000, 64), (3, 333, 2048), (1, 4097, 33)])
+def test_gradients_have_the_same_bits_every_time(B, S, D):
+    ins = on_gpu(*make(B, S, D, BF), grad=True)
+    do = torch.randn(B, S, D, device="cuda").to(BF)
+    first = torch.autograd.grad(gdn2.gated_recurrence(*ins)[0], ins, do)
+    differ = torch.zeros((), dtype=torch.int64, device="cuda")
+    for _ in range(200):
+        for a, b in zip(torch.autograd.grad(gdn2.gated_recurrence(*ins)[0], ins, do), first):
+            differ += (a != b).sum()
+    assert int(differ) == 0
