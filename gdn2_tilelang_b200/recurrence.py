@@ -102,7 +102,7 @@ def gated_recurrence(v, g, w=None, initial_state=None, output_final_state=False,
     A backward pass that is captured into a CUDA graph follows PyTorch's rule for it: no other graph of the same leaves alive
     on another stream (``torch.autograd.grad`` on inputs made for the capture is safe).
     """
-    if g.is_floating_point():                          # (float() of a float32 tensor is the tensor)
+    if g.dtype is not torch.float32 and g.is_floating_point():
         g = g.float()
     if initial_state is not None and initial_state.is_floating_point():
         initial_state = initial_state.float()
@@ -142,7 +142,7 @@ def gated_recurrence_decode(v, g, w, state):
     """Decode ``n`` tokens (``[B, n, ...]``), updating ``state [B, ...]`` (float32, contiguous) in place. ``w`` may be ``None``.
 
     Returns ``o [B, n, ...]`` in ``v.dtype``. No gradient."""
-    if g.is_floating_point():
+    if g.dtype is not torch.float32 and g.is_floating_point():
         g = g.float()
     if v.is_cuda:
         res = _plain(v, g, w, state, True, in_place=True)
