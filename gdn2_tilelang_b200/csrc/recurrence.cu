@@ -12,11 +12,12 @@
 // input is read once and every output written once: a block keeps its tile on chip while the runs are composed. At the copy rate an
 // SM has 55 instructions to spend on a channel and token, which decides the layout: a warp holds 64 channels, two a lane, and
 // eight consecutive tokens, so a lane composes its run alone with packed arithmetic and nothing is shuffled; tiles come by TMA.
-// (Eight channels a lane, composed over the warp by shuffles and fed by a thread's own asynchronous copies, took 52
-// instructions and was bound by them: 153 us for 4 x 4096 x 2048 channels.)
+// It takes 29 forward and 50 backward. (Eight channels a lane, composed over the warp by shuffles and fed by a thread's own
+// asynchronous copies, took 52 forward and was bound by them: 153 us for 4 x 4096 x 2048 channels, bf16, against 59 = 0.86 of the copy
+// rate; backward 252 against 100 = 0.92.)
 //
 // One block walking a sequence would leave most SMs idle (a batch of 2 with 2048 channels is 64 blocks of 64 channels), so a
-// cluster of up to 8 blocks takes as many tiles of the same channels at a time: every block sends the run of its tile to the
+// cluster of up to 16 blocks takes as many tiles of the same channels at a time: every block sends the run of its tile to the
 // others (8 bytes a channel through distributed shared memory, counted by an mbarrier), and each composes what stands before it. The
 // order of composition depends on the sizes only: results are the same bits on every run. Blocks' next tiles are on their way
 // meanwhile, and several blocks share an SM, because composing is latency: two barriers and the exchange a tile.
@@ -25,6 +26,7 @@
 // training step leaves the state that enters every 64th token ("marks", 1/16 byte a channel and token) and the backward pass
 // composes the 64 tokens of its tile again from there.
 #include <algorithm>
+#include <cmath>
 
 #include "clusters.cuh"
 #include "common.cuh"
@@ -38,7 +40,7 @@ namespace {
 constexpr int kR = 8;               // tokens of a warp
 constexpr int kMark = 64;           // tokens between two marks
 constexpr int kC = 64;              // channels of a block
-constexpr int kMaxCluster = 8;
+constexpr int kMaxCluster = 16;
 constexpr int kMaxStages = 4;
 
 struct Tables {                     // packed sequences, the longest first: which each is, its first token, its length, its first mark
@@ -577,11 +579,15 @@ int places(int per_sm, int cl) {
 // How a scan is laid out: warps of a block, blocks of a cluster, stages of a block's feed: the quickest by this account of it. A
 // cluster takes the tiles of its row a round at a time. A round lasts at least as long as the chain of composing and exchanging it,
 // and as all that the blocks at work move in it takes at the copy rate (6500 bytes a nanosecond). Rows that find no place wait for
-// the next wave; a wave starts and ends in 3 us. Packed sequences are of many lengths: the longest alone, all at the copy rate, or
-// all one after another in the places there are, whichever is longest (ten of 16037 tokens together, 2048 channels: clusters of 1
-// 88 us, the longest sequence's chain; as chosen 62). Chains as measured on one row, in us: forward 0.95 with 8 warps, 1.45 with 16,
-// backward 1.85 and 2.8, in clusters 0.2 and 0.02 a block more. Against measurements, forward, bf16, in us: 2 x 4096 x 2048 channels,
-// 8 warps, clusters of 1, 2, 4: 64, 43, 29 and 65, 44, 32; 16 x 4096 x 1024, 8 and 16 warps: 106, 111 and 119, 112.
+// the next wave; a wave starts and ends in 3 us. Backward, and where sequences are of many lengths, an SM's instructions bound it,
+// too, and blocks that share one take their tiles in turn: the busiest SM's where all run at once, the average SM's where they
+// follow one another. Measured, bf16 with a gate, in us, forward and backward: chain of one row 0.95 and 1.85 with 8 warps, 1.45 and 2.8 with 16 (tiles of twice the tokens); in clusters 0.25 and 0.06 a
+// block more, with 16 warps 0.2 and 0.02; an SM's tile 0.93 and 2.0, with 16 warps 1.7 and 3.1. Against measurements, backward:
+// 4 x 4096 x 2048 channels, 8 warps in clusters of 2, 16 warps alone: 131, 102 and 129, 100; 16 x 4096 x 1024, 8 warps alone and in
+// clusters of 4, 16 warps alone: 259, 224, 203 and 269, 212, 217; forward: 2 x 4096 x 2048, 8 warps, clusters of 1, 2, 4: 64, 44, 33 and
+// 65, 44, 32. Packed sequences are of many lengths: the longest alone, all at the copy rate, or all one after another in the
+// places there are, whichever is longest (ten of 16037 tokens together, 2048 channels: clusters of 1 88 us, the longest sequence's
+// chain; as chosen 61).
 struct Layout {
   int warps, cluster, stages;
   size_t smem;
@@ -594,13 +600,14 @@ Layout layout(int64_t rows, int64_t longest, double average, size_t token_bytes,
     const size_t stage = fed ? tile * token_bytes : 0;
     const size_t fixed = (size_t)(back ? 2 * W : W + 1) * 512 + 512;          // a block's Shared
     const int64_t tiles = (longest + tile - 1) / tile;
-    for (int cl = 1; cl <= kMaxCluster && (cl == 1 || cl <= tiles); ++cl) {
+    for (int cl = 1; cl <= kMaxCluster && (cl == 1 || cl <= tiles); cl += cl < kMaxPortableCluster ? 1 : 4) {
       const size_t slots = (size_t)2 * cl * 32 * sizeof(float4);
       for (int per_sm = W > 8 ? 1 : back ? 2 : 3; per_sm >= 1; --per_sm) {     // the kernels' launch bounds, or fewer blocks and more stages
         const size_t room = (size_t)228 * 1024 / per_sm - 1024 - fixed - slots;
         if (room < 2 * stage) continue;
         const int64_t most = places(per_sm, cl);
-        const double chain = (back ? (W > 8 ? 2.8 : 1.85) : (W > 8 ? 1.45 : 0.95)) + (cl > 1 ? 0.2 + 0.02 * cl : 0.0) + (fed ? 0.0 : 1.2);
+        const double chain = (back ? (W > 8 ? 2.8 : 1.85) : (W > 8 ? 1.45 : 0.95)) + (cl > 1 ? (W > 8 ? 0.2 + 0.02 * cl : 0.25 + 0.06 * cl) : 0.0) +
+                             (fed ? 0.0 : 1.2);
         const int64_t rounds = (tiles + cl - 1) / cl;
         double cost;
         if (average == (double)longest) {
@@ -614,6 +621,12 @@ Layout layout(int64_t rows, int64_t longest, double average, size_t token_bytes,
           const double alone = rounds * chain + 3.0, shared = (double)rows / most * (mean * chain + 3.0);
           cost = bytes > alone ? bytes : alone;
           cost = (cost > shared ? cost : shared) + 3.0;
+        }
+        if (back || average != (double)longest) {
+          const double blocks = (double)rows * cl, sms = device_sm_count(), of_tile = back ? (W > 8 ? 3.1 : 2.0) : (W > 8 ? 1.7 : 0.93);
+          const double busiest = blocks <= per_sm * sms ? std::ceil(blocks / sms) : blocks / sms;
+          const double of_sm = busiest * ((average + tile * cl - 1) / (tile * cl)) * of_tile + 3.0;
+          if (of_sm > cost) cost = of_sm;
         }
         if (best.warps == 0 || cost < 0.99 * least) {
           least = cost;
@@ -665,6 +678,7 @@ int launch_scan(const Args& a0, const Tables& tb, int64_t longest, double averag
   if constexpr (Fed)
     if (l.warps > 8) kernel = backward ? scan_backward_kernel<T, 16, Gate, Packed, true> : scan_forward_kernel<T, 16, Gate, Packed, true>;
   GDN2_CUDA_TRY(ensure_dynamic_smem(reinterpret_cast<const void*>(kernel), l.smem));
+  if (l.cluster > kMaxPortableCluster) GDN2_CUDA_TRY(allow_large_clusters(reinterpret_cast<const void*>(kernel)));
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = l.cluster;
