@@ -8,7 +8,7 @@
 //
 // Every product is the same pipeline with another way in and another way out (product_kernel): a pair of blocks on two SMs
 // (cta_group::2) holds a 256 x 256 tile of the result in tensor memory, 128 rows each; TMA brings 64 reduction steps of both
-// operands a stage, each block its own 128 rows of A and its half of B's, six stages deep; one thread issues the products;
+// operands a stage, each block its own 128 rows of A and its half of B's, six stages deep (four where gradients need the room); one thread issues the products;
 // eight warps take the finished tile from tensor memory while the next one accumulates in the other half of it. The operands are read
 // as they lie in memory: with the reduction along rows (K-major) or down columns (MN-major), which the shared-memory
 // descriptors tell the tensor core, so nothing is transposed.
@@ -148,7 +148,7 @@ template <typename T> __host__ __device__ constexpr uint32_t idesc_of(bool a_mn,
 
 // act(a) and, where wanted, act'(a). Both are a times a logistic function: silu s(a), gelu's tanh form s(2 z) with
 // z = sqrt(2 / pi) (a + 0.044715 a^3). Beyond |a| = 16 the latter is 0 or 1 to 32 bits; z stops there so that a^3 stays finite.
-// (A template argument: with a branch on it inside the epilogue's loops the backward one took twice as long as its products.)
+// (A template argument: with a branch on it inside the epilogue's loops the backward one took 250 us instead of 209, 8192 x 2048 x 5632.)
 // The exponential and the reciprocal are the approximate instructions: 2^-21, against results of 11 bits at most.
 __device__ __forceinline__ float logistic(float x) { return __fdividef(1.f, 1.f + __expf(-x)); }
 template <bool Gelu, bool Slope> __device__ __forceinline__ float activate(float a, float& slope) {
@@ -575,7 +575,7 @@ product_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Proble
         }
       } else {
         // a piece's a and u go to registers, the next piece's are asked for, and only then the work on them begins: the load's latency
-        // and the stores' are both behind it (loading after the stores of the piece before: 250 us instead of 209 for 8192 x 2048 x 5632)
+        // and the stores' are both behind it (pieces of 64 columns loaded after the stores before them: 209 us instead of 203, 8192 x 2048 x 5632)
         bool ok = true;
         char* out = chunk + 6144;
 #pragma unroll 1

@@ -581,8 +581,8 @@ int places(int per_sm, int cl) {
 // and as all that the blocks at work move in it takes at the copy rate (6500 bytes a nanosecond). Rows that find no place wait for
 // the next wave; a wave starts and ends in 3 us. Backward, and where sequences are of many lengths, an SM's instructions bound it,
 // too, and blocks that share one take their tiles in turn: the busiest SM's where all run at once, the average SM's where they
-// follow one another. Measured, bf16 with a gate, in us, forward and backward: chain of one row 0.95 and 1.85 with 8 warps, 1.45 and 2.8 with 16 (tiles of twice the tokens); in clusters 0.25 and 0.06 a
-// block more, with 16 warps 0.2 and 0.02; an SM's tile 0.93 and 2.0, with 16 warps 1.7 and 3.1. Against measurements, backward:
+// follow one another. Measured, bf16 with a gate, in us, forward and backward: chain of one row 0.95 and 1.85 with 8 warps, 1.45 and
+// 2.8 with 16 (tiles of twice the tokens); in clusters 0.25 and 0.06 a block more, with 16 warps 0.2 and 0.02; an SM's tile 0.93 and 2.0, with 16 warps 1.7 and 3.1. Against measurements, backward:
 // 4 x 4096 x 2048 channels, 8 warps in clusters of 2, 16 warps alone: 131, 102 and 129, 100; 16 x 4096 x 1024, 8 warps alone and in
 // clusters of 4, 16 warps alone: 259, 224, 203 and 269, 212, 217; forward: 2 x 4096 x 2048, 8 warps, clusters of 1, 2, 4: 64, 44, 33 and
 // 65, 44, 32. Packed sequences are of many lengths: the longest alone, all at the copy rate, or all one after another in the
