@@ -127,7 +127,12 @@ def gated_recurrence(v, g, w=None, initial_state=None, output_final_state=False,
             return res
     if v.numel() == 0:                                 # nothing to compute: the states pass through
         final = torch.zeros(N, *channels, dtype=torch.float32, device=v.device) if initial_state is None else initial_state.clone()
-        return torch.empty_like(v, memory_format=torch.contiguous_format), (final if output_final_state else None)
+        o = torch.empty_like(v, memory_format=torch.contiguous_format)
+        ins = [t for t in (v, g, w, initial_state) if t is not None and t.requires_grad]
+        if torch.is_grad_enabled() and ins:            # zero gradients, from sums of no elements
+            nothing = sum(t[:0].sum() for t in ins)
+            o, final = o.detach() + nothing.to(o.dtype), final + nothing.float()
+        return o, (final if output_final_state else None)
     rows = [None if t is None else t.flatten(2) for t in (v, g, w)]
     state = None if initial_state is None else initial_state.reshape(N, -1)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (v, g, w, initial_state)):
