@@ -505,6 +505,18 @@ template <int VEC> __device__ __forceinline__ void load_f32(float (&x)[VEC], con
     }
   }
 }
+// A state, which the same launch may write: by ordinary loads, not by those for data that nothing writes meanwhile
+template <int VEC> __device__ __forceinline__ void load_state(float (&x)[VEC], const float* p) {
+  if constexpr (VEC == 1) {
+    x[0] = *p;
+  } else {
+#pragma unroll
+    for (int i = 0; i < VEC; i += 4) {
+      const float4 r = *reinterpret_cast<const float4*>(p + i);
+      x[i] = r.x; x[i + 1] = r.y; x[i + 2] = r.z; x[i + 3] = r.w;
+    }
+  }
+}
 template <int VEC> __device__ __forceinline__ void store_f32(float* p, const float (&x)[VEC]) {
   if constexpr (VEC == 1) {
     *p = x[0];
@@ -539,7 +551,7 @@ __global__ void __launch_bounds__(128) scan_steps_kernel(const __grid_constant__
   const T* w = Gate ? static_cast<const T*>(a.w) + seq * a.w_bs + c0 : nullptr;
   const float* g = a.g + seq * a.g_bs + c0;
   T* o = static_cast<T*>(a.o) + seq * a.S * a.D + c0;
-  if (a.first) load_f32<VEC>(h, a.first + seq * a.D + c0);
+  if (a.first) load_state<VEC>(h, a.first + seq * a.D + c0);
   constexpr int kAhead = 4;                           // tokens in flight
   const int S = (int)a.S;
   for (int t0 = 0; t0 < S; t0 += kAhead) {
@@ -582,8 +594,8 @@ int places(int per_sm, int cl) {
 // the next wave; a wave starts and ends in 3 us. Backward, and where sequences are of many lengths, an SM's instructions bound it,
 // too, and blocks that share one take their tiles in turn: the busiest SM's where all run at once, the average SM's where they
 // follow one another. Measured, bf16 with a gate, in us, forward and backward: chain of one row 0.95 and 1.85 with 8 warps, 1.45 and
-// 2.8 with 16 (tiles of twice the tokens); in clusters 0.25 and 0.06 a block more, with 16 warps 0.2 and 0.02; an SM's tile 0.93 and 2.0, with 16 warps 1.7 and 3.1. Against measurements, backward:
-// 4 x 4096 x 2048 channels, 8 warps in clusters of 2, 16 warps alone: 131, 102 and 129, 100; 16 x 4096 x 1024, 8 warps alone and in
+// 2.8 with 16 (tiles of twice the tokens); in clusters 0.25 and 0.06 a block more, with 16 warps 0.2 and 0.02; an SM's tile 0.93 and 2.0, with 16
+// warps 1.7 and 3.1. Against measurements, backward: 4 x 4096 x 2048 channels, 8 warps in clusters of 2, 16 warps alone: 131, 102 and 129, 100; 16 x 4096 x 1024, 8 warps alone and in
 // clusters of 4, 16 warps alone: 259, 224, 203 and 269, 212, 217; forward: 2 x 4096 x 2048, 8 warps, clusters of 1, 2, 4: 64, 44, 33 and
 // 65, 44, 32. Packed sequences are of many lengths: the longest alone, all at the copy rate, or all one after another in the
 // places there are, whichever is longest (ten of 16037 tokens together, 2048 channels: clusters of 1 88 us, the longest sequence's
