@@ -120,6 +120,10 @@ __device__ __forceinline__ void commit_pair(uint64_t* bar, uint32_t leader) {
   asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
                ::"r"(tc::smem_u32(bar)), "h"((uint16_t)(3u << leader)) : "memory");
 }
+// A lane has read what it will of the memory that this barrier stands for: the arrival comes after its loads
+__device__ __forceinline__ void arrive_read(uint64_t* bar) {
+  asm volatile("mbarrier.arrive.release.cta.shared::cta.b64 _, [%0];" ::"r"(tc::smem_u32(bar)) : "memory");
+}
 __device__ __forceinline__ void arrive_remote(uint32_t bar) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
@@ -242,15 +246,6 @@ __device__ __forceinline__ void get_kept(const char* upper, const char* lower, i
     }
   }
 }
-// Uses what get_kept has read, an instruction for each of its loads: loads from shared memory may wait their turn behind the warps'
-// other accesses for longer than a copy takes to arrive, so one that overwrites the piece may only be asked for when the values
-// have come back. (Without it, and with more of them waiting, an a or u in some tens of calls was the next piece's.)
-__device__ __forceinline__ void in_registers(const float (&x)[32]) {
-  uint32_t s = 0;
-#pragma unroll
-  for (int i = 0; i < 32; i += 4) s ^= __float_as_uint(x[i]);
-  asm volatile("" ::"r"(s) : "memory");
-}
 // A warp's chunk to rows row.., columns col.. of the result; what lies outside is dropped.
 template <typename T>
 __device__ __forceinline__ void store_chunk(const char* chunk, const CUtensorMap* map, T* plain, int64_t stride, int row, int col, int M,
@@ -282,7 +277,7 @@ __device__ __forceinline__ void chunk_free(int lane) {        // the chunk may b
 // ---------------------------------------------------------------- tiles of 256 x 256
 
 struct Shared {
-  uint64_t full[8], empty[8], done[2], taken[2], loaded[kEpiWarps];
+  uint64_t full[8], empty[8], done[2], taken[2], loaded[kEpiWarps], read[kEpiWarps];
   uint32_t tmem;
   int abort;
 };
@@ -407,7 +402,10 @@ product_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Proble
       tc::mbar_init(&sh.done[i], 1);
       tc::mbar_init(&sh.taken[i], 2 * kEpiWarps);
     }
-    for (int i = 0; i < kEpiWarps; ++i) tc::mbar_init(&sh.loaded[i], 1);
+    for (int i = 0; i < kEpiWarps; ++i) {
+      tc::mbar_init(&sh.loaded[i], 1);
+      tc::mbar_init(&sh.read[i], 32);
+    }
     sh.abort = 0;
     tc::mbar_init_fence();
   }
@@ -587,10 +585,14 @@ product_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Proble
           tc::tmem_ld32(acc + half * 128 + 32 * c, d);
           get_kept(chunk, chunk + 4096, lane, a);
           get_kept(chunk + 2048, chunk + 5120, lane, u);
-          in_registers(a);
-          in_registers(u);
+          // Every lane's loads of the piece come before the copy that overwrites it: a load from shared memory may wait its turn behind
+          // the warps' other accesses for longer than a copy takes to arrive, and neither a warp barrier nor an asm statement without
+          // an instruction holds the copy back (an a or u in some tens of calls was the next piece's). Arrivals of all lanes do.
+          arrive_read(&sh.read[ew]);
+          if (lane == 0 && tc::mbar_wait(&sh.read[ew], (loads - 1) & 1, &sh.abort, status, kWaitCode)) {
+            if (c < 3) load_piece(i, c + 1); else load_piece(i + pairs, 0);
+          }
           __syncwarp();
-          if (c < 3) load_piece(i, c + 1); else load_piece(i + pairs, 0);
           tc::tmem_ld_wait();
           float h[32];
 #pragma unroll
