@@ -30,7 +30,9 @@ uint32_t* device_status_word() {
   return static_cast<uint32_t*>(p);
 }
 
-// cudaFuncSetAttribute(MaxDynamicSharedMemorySize) sticks to a (kernel, device) pair: made once, not on every launch
+// cudaFuncSetAttribute(MaxDynamicSharedMemorySize) sticks to a (kernel, device) pair: made once, not on every launch. Calls of one kernel
+// ask for different sizes, from several threads: the limit is looked up, raised and noted under one lock, and never lowered, because
+// another thread may be about to launch with what it was promised.
 cudaError_t ensure_dynamic_smem(const void* kernel, size_t bytes) {
   static std::mutex mu;
   static std::unordered_map<unsigned long long, size_t> done;
@@ -38,16 +40,11 @@ cudaError_t ensure_dynamic_smem(const void* kernel, size_t bytes) {
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
   const unsigned long long key = reinterpret_cast<unsigned long long>(kernel) ^ (static_cast<unsigned long long>(dev) << 56);
-  {
-    std::lock_guard<std::mutex> lk(mu);
-    auto it = done.find(key);
-    if (it != done.end() && it->second >= bytes) return cudaSuccess;
-  }
+  std::lock_guard<std::mutex> lk(mu);
+  size_t& most = done[key];
+  if (most >= bytes) return cudaSuccess;
   e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
-  if (e == cudaSuccess) {
-    std::lock_guard<std::mutex> lk(mu);
-    done[key] = bytes;
-  }
+  if (e == cudaSuccess) most = bytes;
   return e;
 }
 
