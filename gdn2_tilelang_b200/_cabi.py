@@ -357,7 +357,7 @@ class NativeKernels:
             rc = fn(q.data_ptr(), k.data_ptr(), v.data_ptr(), g.data_ptr(), b.data_ptr(), w.data_ptr(), state.data_ptr(),
                     o.data_ptr(), B, n, H, HK, DK, DV, in_bs, o_bs, float(scale), code, self._stream(q))
         _check(self.lib, rc, "gdn2_decode")
-        self.launches += 1
+        self._launches += 1
         return o
 
     def prefill_plain(self, q, k, v, g, b, w, scale, state):
@@ -366,7 +366,7 @@ class NativeKernels:
         res = self.host.prefill(q, k, v, g, b, w, scale, state, self.prefill_path, side)
         if res is None:
             return None
-        self.launches += res[2]
+        self._launches += res[2]
         return res[0], res[1]
 
     # -- prefill in one call ---------------------------------------------------------------
@@ -410,7 +410,7 @@ class NativeKernels:
                 ws.data_ptr(), nbytes, B, S, H, HK, DK, DV, in_bs, S, float(scale), code, p,
                 None if side is None else side.cuda_stream, main.cuda_stream)
         _check(self.lib, rc, "gdn2_prefill_ragged")
-        self.launches += (2 if p != PATH_SIMT else 1) + self.lib.gdn2_prefill_scan_launches(B, n_full, H, DK, DV, code, p) \
+        self._launches += (2 if p != PATH_SIMT else 1) + self.lib.gdn2_prefill_scan_launches(B, n_full, H, DK, DV, code, p) \
             + (1 if S > n_full and p != PATH_SIMT else 0)
         return o, final_state
 
@@ -441,7 +441,7 @@ class NativeKernels:
                 None if initial_state is None else initial_state.data_ptr(), o.data_ptr(), final_state.data_ptr(),
                 ws.data_ptr(), nbytes, H, HK, DK, DV, float(scale), code, p, self._stream(q))
         _check(self.lib, rc, "gdn2_packed_forward")
-        self.launches += self.lib.gdn2_packed_launches(cu, N, H, HK, DK, DV, code, p)
+        self._launches += self.lib.gdn2_packed_launches(cu, N, H, HK, DK, DV, code, p)
         return o, final_state
 
     # -- chunkwise forward -----------------------------------------------------------------
@@ -563,7 +563,7 @@ class NativeKernels:
             if side is not None:
                 main.wait_stream(side)             # from here on the caller's stream is ordered after every scan
             del scratch                            # ... so only now may the allocator hand these blocks out again
-        self.launches += launched
+        self._launches += launched
         if then_with_state is not None:
             then_with_state(final_state)
         return out, final_state, hs
@@ -588,7 +588,7 @@ class NativeKernels:
             rc = self.lib.gdn2_chunk_output(ws.data_ptr(), nbytes, chunk_states.data_ptr(), out.data_ptr(),
                                             B, S, H, HK, DK, DV, S, code, p, st)
             _check(self.lib, rc, "gdn2_chunk_output")
-        self.launches += 3 if p != PATH_SIMT else 2
+        self._launches += 3 if p != PATH_SIMT else 2
         return out
 
     # -- diagonal recurrence -----------------------------------------------------------------
@@ -634,7 +634,7 @@ class NativeKernels:
         with _on_device(dev):
             rc = self.lib.gdn2_recurrence_forward(ctypes.byref(a), dtype_code(v.dtype), self._stream(v))
         _check(self.lib, rc, "gdn2_recurrence_forward")
-        self.launches += self._recurrence_launches(a)
+        self._launches += self._recurrence_launches(a)
         return o, final, marks
 
     def recurrence_backward(self, v, g, w, marks, do, dfinal, offsets, want_dstate):
@@ -653,7 +653,7 @@ class NativeKernels:
         with _on_device(dev):
             rc = self.lib.gdn2_recurrence_backward(ctypes.byref(a), dtype_code(v.dtype), self._stream(v))
         _check(self.lib, rc, "gdn2_recurrence_backward")
-        self.launches += self._recurrence_launches(a)
+        self._launches += self._recurrence_launches(a)
         return dv, dg, dw, dstate
 
     # -- gated feed-forward ------------------------------------------------------------------
@@ -673,7 +673,7 @@ class NativeKernels:
             with _on_device(out[0].device):
                 rc = self.lib.gdn2_align_rows((RowCopy * len(copies))(*copies), len(copies), self._stream(out[0]))
             _check(self.lib, rc, "gdn2_align_rows")
-            self.launches += 1
+            self._launches += 1
         return out
 
     @staticmethod
@@ -698,7 +698,7 @@ class NativeKernels:
         with _on_device(x.device):
             rc = self.lib.gdn2_ffn_forward(ctypes.byref(a), dtype_code(x.dtype), self._stream(x))
         _check(self.lib, rc, "gdn2_ffn_forward")
-        self.launches += 2
+        self._launches += 2
         return y, kept
 
     def ffn_backward(self, x, w_gate, w_up, w_down, kept, dy, activation: str, want_dx: bool, want_dgate_up: bool, want_dw_down: bool):
@@ -715,7 +715,7 @@ class NativeKernels:
         with _on_device(x.device):
             rc = self.lib.gdn2_ffn_backward(ctypes.byref(a), dtype_code(x.dtype), self._stream(x))
         _check(self.lib, rc, "gdn2_ffn_backward")
-        self.launches += 1 + int(want_dx) + int(want_dgate_up) + int(want_dw_down)
+        self._launches += 1 + int(want_dx) + int(want_dgate_up) + int(want_dw_down)
         return dx, dwg, dwu, dwd
 
     # -- diagnostics -------------------------------------------------------------------------
@@ -774,7 +774,7 @@ class NativeKernels:
         with _on_device(dev):
             rc = self.lib.gdn2_layer_front(ctypes.byref(a), dtype_code(dt), self._stream(proj))
         _check(self.lib, rc, "gdn2_layer_front")
-        self.launches += 2 if (new_conv is not None and not self._layer_front_is_one_kernel(proj, offsets, DK, DV, K)) else 1
+        self._launches += 2 if (new_conv is not None and not self._layer_front_is_one_kernel(proj, offsets, DK, DV, K)) else 1
         return q, k, v, g, b, w, new_conv
 
     def layer_step(self, x, state, conv_state, w_cat, conv_weight, conv_bias, A_log, dt_bias, norm_weight, o_weight, offsets, H, HK,
@@ -822,7 +822,7 @@ class NativeKernels:
                                           B * S, H, DV, proj.shape[-1], off_gate, eps, dtype_code(o.dtype),
                                           self._stream(o))
         _check(self.lib, rc, "gdn2_layer_back")
-        self.launches += 1
+        self._launches += 1
         return out
 
     def maybe_check_device_status(self, device):
@@ -857,7 +857,7 @@ class NativeKernels:
                                           w.data_ptr(), ws.data_ptr(), nbytes, B, S, H, HK, DK, DV, S, float(scale),
                                           code, p, self._stream(q))
         _check(self.lib, rc, "gdn2_chunk_prep")
-        self.launches += 2 if p != PATH_SIMT else 1
+        self._launches += 2 if p != PATH_SIMT else 1
         return ws, p
 
     def oproj_reduce(self, x, weight, out, peer_slots, peer_flags, epochs, rank, world, wait_cycles=0):
@@ -872,7 +872,7 @@ class NativeKernels:
         with _on_device(x.device):
             rc = self.lib.gdn2_oproj_reduce(ctypes.byref(a), dtype_code(x.dtype), self._stream(x))
         _check(self.lib, rc, "gdn2_oproj_reduce")
-        self.launches += 1
+        self._launches += 1
         return out
 
     def selftest_wait(self, limit_cycles: int, device=None) -> int:

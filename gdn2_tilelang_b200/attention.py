@@ -320,7 +320,7 @@ class GatedDeltaNet2(nn.Module):
         out, conv, launched = res
         if not conv_in_place:
             cache.conv_state = conv
-        K.launches += launched
+        K._launches += launched
         K.maybe_check_device_status(x.device)
         return out
 
@@ -335,7 +335,7 @@ class GatedDeltaNet2(nn.Module):
         if res is None:
             return None
         out, cache.recurrent_state, cache.conv_state, launched = res
-        K.launches += launched
+        K._launches += launched
         K.maybe_check_device_status(x.device)
         return out
 

@@ -48,7 +48,7 @@ def _decode_plain(q, k, v, g, b, w, state, scale):
     host = getattr(K, "host", None)
     o = None if host is None else host.decode(q, k, v, g, b, w, state, scale)
     if o is not None:
-        K.launches += 1
+        K._launches += 1
         K.maybe_check_device_status(q.device)
     return o
 
@@ -89,7 +89,7 @@ def _prefill_short(q, k, v, g, b, w, state, scale):
     call = getattr(getattr(K, "host", None), "prefill_short", None)
     res = None if call is None else call(q, k, v, g, b, w, scale, state)
     if res is not None:
-        K.launches += 1
+        K._launches += 1
         K.maybe_check_device_status(q.device)
     return res
 
