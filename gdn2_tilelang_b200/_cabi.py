@@ -19,6 +19,7 @@ import threading
 import warnings
 
 import torch
+from torch.autograd import forward_ad
 
 _PKG = pathlib.Path(__file__).resolve().parent
 _LIB_PATH = _PKG / "libgdn2_b200.so"
@@ -243,6 +244,13 @@ def _seq_view(t: torch.Tensor):
             return t, (t.stride(0) // (H * D) if B > 1 else S)
     t = t.contiguous()
     return t, S
+
+
+def refuse_tangents(what: str, *tensors):
+    """The kernels are launched outside autograd's sight, and their operators have a gradient in reverse mode alone: an input with a
+    forward-mode tangent is refused, because the result would silently have none."""
+    if torch._C._is_fwd_grad_enabled() and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise NotImplementedError(f"{what} has no forward-mode derivative (an input carries a tangent); differentiate it in reverse mode")
 
 
 def _rows_view(t: torch.Tensor):

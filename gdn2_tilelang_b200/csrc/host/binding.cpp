@@ -10,6 +10,7 @@
 #include <ATen/ATen.h>
 #include <ATen/autocast_mode.h>
 #include <ATen/core/grad_mode.h>
+#include <c10/core/AutogradState.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAGuard.h>
@@ -305,6 +306,18 @@ bool wants_grad(std::initializer_list<const Tensor*> ts) {
     if (t->defined() && t->requires_grad()) return true;
   return false;
 }
+// An input with a forward-mode tangent: the operators have none, and the general path says so
+bool has_tangent(std::initializer_list<const Tensor*> ts) {
+  if (!c10::AutogradState::get_tls_state().get_fw_grad_mode()) return false;
+  for (const Tensor* t : ts)
+    if (t->defined() && t->_fw_grad(0).defined()) return true;
+  return false;
+}
+// A gradient with a tangent (forward mode over reverse mode)
+void refuse_tangents(const variable_list& grads, const char* what) {
+  for (const Tensor& t : grads)
+    TORCH_CHECK_NOT_IMPLEMENTED(!has_tangent({&t}), what, " has no forward-mode derivative (a gradient carries a tangent)");
+}
 // Gradients that were asked for with create_graph: there is no second derivative, and using one says so.
 variable_list once(variable_list grads, const char* what) {
   if (!at::GradMode::is_enabled()) return grads;
@@ -365,6 +378,7 @@ struct Recurrence : torch::autograd::Function<Recurrence> {
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     if (!grads[0].defined() && !grads[1].defined()) return variable_list(5);
+    refuse_tangents(grads, "gated_recurrence");
     const auto saved = ctx->get_saved_variables();
     variable_list out(5);
     {
@@ -408,6 +422,7 @@ std::optional<std::tuple<Tensor, std::optional<Tensor>, int64_t>> recurrence(con
   if (state && (!unwrapped(*state, at::kFloat, dev) || !state->is_contiguous() || state->sizes() != at::IntArrayRef(state_shape)))
     return std::nullopt;
   const Tensor s = state ? state->view({sequences, -1}) : Tensor();
+  if (has_tangent({&vr, &gr, &wr, &s})) return std::nullopt;
   const bool grad = wants_grad({&vr, &gr, &wr, &s});
   if (in_place && (grad || !state)) return std::nullopt;
   if (grad) {
@@ -478,6 +493,7 @@ struct FeedForward : torch::autograd::Function<FeedForward> {
     const auto saved = ctx->get_saved_variables();
     variable_list out(5);
     if (!grads[0].defined()) return out;
+    refuse_tangents(grads, "gated_feed_forward");
     {
       at::NoGradGuard no_grad;
       const std::vector<Tensor> in(saved.begin(), saved.begin() + 4);
@@ -514,6 +530,7 @@ std::optional<std::tuple<Tensor, int64_t>> feed_forward(const Tensor& x, const T
       !unwrapped(wd, type, dev) || x.dim() < 1 || wg.dim() != 2 || wd.dim() != 2 || wu.sizes() != wg.sizes() || wd.size(1) != wg.size(0) ||
       x.size(-1) != wg.size(1) || x.numel() == 0 || wg.numel() == 0 || wd.numel() == 0 || !(x.dim() == 2 || x.is_contiguous()))
     return std::nullopt;
+  if (has_tangent({&x, &wg, &wu, &wd})) return std::nullopt;
   const Tensor rows = x.dim() == 2 ? x : x.view({-1, x.size(-1)});
   std::vector<int64_t> shape(x.sizes().begin(), x.sizes().end());
   shape.back() = wd.size(0);

@@ -54,6 +54,7 @@ class _GatedFeedForward(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, dy):
         K = _cabi.kernels()
+        _cabi.refuse_tangents("gated_feed_forward", dy)
         need = ctx.needs_input_grad
         dy = K.aligned_rows(dy)[0]
         dx, dwg, dwu, dwd = K.ffn_backward(*ctx.saved_tensors, dy, ctx.activation, need[0], need[1] or need[2], need[3])
@@ -62,7 +63,7 @@ class _GatedFeedForward(torch.autograd.Function):
 
 
 def gated_feed_forward(x, w_gate, w_up, w_down, activation="silu"):
-    """``(act(x w_gate^T) * (x w_up^T)) w_down^T``; differentiable (once).
+    """``(act(x w_gate^T) * (x w_up^T)) w_down^T``; differentiable in reverse mode, once.
 
     ``x``: ``[..., hidden]``; ``w_gate, w_up``: ``[inner, hidden]``; ``w_down``: ``[out, inner]`` (the layout of ``nn.Linear``), all float16
     or all bfloat16. ``activation``: ``"silu"`` or ``"gelu_tanh"``. Returns ``[..., out]``. What one product
@@ -80,6 +81,7 @@ def gated_feed_forward(x, w_gate, w_up, w_down, activation="silu"):
                 K._launches += res[1]
                 return res[0]
     _check(x, w_gate, w_up, w_down, activation)
+    _cabi.refuse_tangents("gated_feed_forward", x, w_gate, w_up, w_down)
     out_shape = (*x.shape[:-1], w_down.shape[0])
     needs_grad = torch.is_grad_enabled() and any(t.requires_grad for t in (x, w_gate, w_up, w_down))
     if x.numel() == 0:                                 # no tokens: an empty result, zero gradients

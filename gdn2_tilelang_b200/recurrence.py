@@ -64,6 +64,7 @@ class _GatedRecurrence(torch.autograd.Function):
     def backward(ctx, do, dfinal):
         if do is None and dfinal is None:
             return None, None, None, None, None
+        _cabi.refuse_tangents("gated_recurrence", do, dfinal)
         v, g, w, marks = ctx.saved_tensors
         K = _cabi.kernels()
         do = torch.zeros_like(v) if do is None else do
@@ -87,7 +88,8 @@ def _plain(v, g, w, state, want_final, in_place=False, offsets=()):
 
 
 def gated_recurrence(v, g, w=None, initial_state=None, output_final_state=False, cu_seqlens=None):
-    """``h_t = exp(g_t) * h_{t-1} + w_t * v_t`` along the tokens of whole sequences; differentiable (once).
+    """``h_t = exp(g_t) * h_{t-1} + w_t * v_t`` along the tokens of whole sequences; differentiable in
+    reverse mode, once.
 
     ``v, g, w``: ``[B, S, ...]``, one shape; all trailing dimensions are channels. ``v`` and ``w`` are float16, bfloat16 or
     float32, ``g`` (``<= 0``, ``-inf`` forgets the state) is coerced to float32; ``w=None`` writes ``v`` as it is.
@@ -111,6 +113,7 @@ def gated_recurrence(v, g, w=None, initial_state=None, output_final_state=False,
         if res is not None:
             return res
     _check_rows(v, g, w)
+    _cabi.refuse_tangents("gated_recurrence", v, g, w, initial_state)
     B, S = v.shape[:2]
     channels = tuple(v.shape[2:])
     offsets = None if cu_seqlens is None else _offsets(cu_seqlens, v)
@@ -154,6 +157,7 @@ def gated_recurrence_decode(v, g, w, state):
         if res is not None:
             return res[0]
     _check_rows(v, g, w)
+    _cabi.refuse_tangents("gated_recurrence_decode", v, g, w, state)
     B = v.shape[0]
     if tuple(state.shape) != (B, *v.shape[2:]):
         raise ValueError(f"state must have shape {(B, *v.shape[2:])}, got {tuple(state.shape)}")
