@@ -253,6 +253,15 @@ def refuse_tangents(what: str, *tensors):
         raise NotImplementedError(f"{what} has no forward-mode derivative (an input carries a tangent); differentiate it in reverse mode")
 
 
+def refuse_tracing(what: str):
+    """A tracer records operators that go through PyTorch's dispatcher; of a kernel it would record the empty result alone."""
+    keys = torch._C._TorchDispatchModeKey
+    if (torch.jit.is_tracing() or torch._ops._len_torch_dispatch_stack_pre_dispatch() > 0
+            or any(torch._C._get_dispatch_mode(k) is not None for k in (keys.PROXY, keys.FAKE, keys.FUNCTIONAL))):
+        raise NotImplementedError(f"{what} cannot be traced (make_fx, export, jit.trace, fake tensors): its kernel is not an operator that "
+                                  "a tracer sees; call it outside the traced function")
+
+
 def _rows_view(t: torch.Tensor):
     """``(tensor, batch stride, token stride)`` in elements of ``[B, S, D]`` rows whose channels lie side by side; copied if
     they do not. The stride of a dimension of one entry is never used and given as 0."""

@@ -8,6 +8,7 @@
 #include <atomic>
 
 #include <ATen/ATen.h>
+#include <ATen/TracerMode.h>
 #include <ATen/autocast_mode.h>
 #include <ATen/core/grad_mode.h>
 #include <c10/core/AutogradState.h>
@@ -313,8 +314,17 @@ bool has_tangent(std::initializer_list<const Tensor*> ts) {
     if (t->defined() && t->_fw_grad(0).defined()) return true;
   return false;
 }
-// A gradient with a tangent (forward mode over reverse mode)
-void refuse_tangents(const variable_list& grads, const char* what) {
+// A tracer is at work, which would record the empty result of a kernel alone
+bool traced() {
+  using c10::impl::TorchDispatchModeTLS;
+  using Key = c10::impl::TorchDispatchModeKey;
+  if (at::tracer::impl::is_dispatch_enabled() || c10::impl::tls_is_dispatch_key_included(c10::DispatchKey::PreDispatch)) return true;
+  return TorchDispatchModeTLS::any_modes_set() &&
+         (TorchDispatchModeTLS::get_mode(Key::PROXY) || TorchDispatchModeTLS::get_mode(Key::FAKE) || TorchDispatchModeTLS::get_mode(Key::FUNCTIONAL));
+}
+// A backward pass that is traced, or whose gradients carry tangents (forward mode over reverse mode)
+void refuse_transforms(const variable_list& grads, const char* what) {
+  TORCH_CHECK_NOT_IMPLEMENTED(!traced(), what, " cannot be traced: its gradient's kernels are not operators that a tracer sees");
   for (const Tensor& t : grads)
     TORCH_CHECK_NOT_IMPLEMENTED(!has_tangent({&t}), what, " has no forward-mode derivative (a gradient carries a tangent)");
 }
@@ -378,7 +388,7 @@ struct Recurrence : torch::autograd::Function<Recurrence> {
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     if (!grads[0].defined() && !grads[1].defined()) return variable_list(5);
-    refuse_tangents(grads, "gated_recurrence");
+    refuse_transforms(grads, "gated_recurrence");
     const auto saved = ctx->get_saved_variables();
     variable_list out(5);
     {
@@ -422,7 +432,7 @@ std::optional<std::tuple<Tensor, std::optional<Tensor>, int64_t>> recurrence(con
   if (state && (!unwrapped(*state, at::kFloat, dev) || !state->is_contiguous() || state->sizes() != at::IntArrayRef(state_shape)))
     return std::nullopt;
   const Tensor s = state ? state->view({sequences, -1}) : Tensor();
-  if (has_tangent({&vr, &gr, &wr, &s})) return std::nullopt;
+  if (has_tangent({&vr, &gr, &wr, &s}) || traced()) return std::nullopt;
   const bool grad = wants_grad({&vr, &gr, &wr, &s});
   if (in_place && (grad || !state)) return std::nullopt;
   if (grad) {
@@ -493,7 +503,7 @@ struct FeedForward : torch::autograd::Function<FeedForward> {
     const auto saved = ctx->get_saved_variables();
     variable_list out(5);
     if (!grads[0].defined()) return out;
-    refuse_tangents(grads, "gated_feed_forward");
+    refuse_transforms(grads, "gated_feed_forward");
     {
       at::NoGradGuard no_grad;
       const std::vector<Tensor> in(saved.begin(), saved.begin() + 4);
@@ -530,7 +540,7 @@ std::optional<std::tuple<Tensor, int64_t>> feed_forward(const Tensor& x, const T
       !unwrapped(wd, type, dev) || x.dim() < 1 || wg.dim() != 2 || wd.dim() != 2 || wu.sizes() != wg.sizes() || wd.size(1) != wg.size(0) ||
       x.size(-1) != wg.size(1) || x.numel() == 0 || wg.numel() == 0 || wd.numel() == 0 || !(x.dim() == 2 || x.is_contiguous()))
     return std::nullopt;
-  if (has_tangent({&x, &wg, &wu, &wd})) return std::nullopt;
+  if (has_tangent({&x, &wg, &wu, &wd}) || traced()) return std::nullopt;
   const Tensor rows = x.dim() == 2 ? x : x.view({-1, x.size(-1)});
   std::vector<int64_t> shape(x.sizes().begin(), x.sizes().end());
   shape.back() = wd.size(0);

@@ -54,6 +54,7 @@ class _GatedFeedForward(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, dy):
         K = _cabi.kernels()
+        _cabi.refuse_tracing("gated_feed_forward")
         _cabi.refuse_tangents("gated_feed_forward", dy)
         need = ctx.needs_input_grad
         dy = K.aligned_rows(dy)[0]
@@ -81,6 +82,7 @@ def gated_feed_forward(x, w_gate, w_up, w_down, activation="silu"):
                 K._launches += res[1]
                 return res[0]
     _check(x, w_gate, w_up, w_down, activation)
+    _cabi.refuse_tracing("gated_feed_forward")
     _cabi.refuse_tangents("gated_feed_forward", x, w_gate, w_up, w_down)
     out_shape = (*x.shape[:-1], w_down.shape[0])
     needs_grad = torch.is_grad_enabled() and any(t.requires_grad for t in (x, w_gate, w_up, w_down))

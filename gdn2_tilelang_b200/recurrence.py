@@ -64,6 +64,7 @@ class _GatedRecurrence(torch.autograd.Function):
     def backward(ctx, do, dfinal):
         if do is None and dfinal is None:
             return None, None, None, None, None
+        _cabi.refuse_tracing("gated_recurrence")
         _cabi.refuse_tangents("gated_recurrence", do, dfinal)
         v, g, w, marks = ctx.saved_tensors
         K = _cabi.kernels()
@@ -113,6 +114,7 @@ def gated_recurrence(v, g, w=None, initial_state=None, output_final_state=False,
         if res is not None:
             return res
     _check_rows(v, g, w)
+    _cabi.refuse_tracing("gated_recurrence")
     _cabi.refuse_tangents("gated_recurrence", v, g, w, initial_state)
     B, S = v.shape[:2]
     channels = tuple(v.shape[2:])
@@ -157,6 +159,7 @@ def gated_recurrence_decode(v, g, w, state):
         if res is not None:
             return res[0]
     _check_rows(v, g, w)
+    _cabi.refuse_tracing("gated_recurrence_decode")
     _cabi.refuse_tangents("gated_recurrence_decode", v, g, w, state)
     B = v.shape[0]
     if tuple(state.shape) != (B, *v.shape[2:]):

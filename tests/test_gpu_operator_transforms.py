@@ -1,4 +1,4 @@
-"""Forward-mode tangents on the device: the calls that go through the host extension refuse them, too, as inputs and as gradients."""
+"""Forward-mode tangents and tracers on the device: the calls that go through the host extension refuse them, too, forward and backward."""
 
 from __future__ import annotations
 
@@ -67,3 +67,32 @@ def test_a_decoded_token_with_a_tangent():
     with forward_ad.dual_level(), pytest.raises(NotImplementedError, match="forward-mode"):
         gdn2.gated_recurrence_decode(forward_ad.make_dual(g, torch.ones_like(g)), g, None, state)
     assert not state.any()
+
+
+@pytest.mark.parametrize("name", MAKE)
+def test_a_trace(name):
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    call, ins = MAKE[name]()
+    with pytest.raises(NotImplementedError, match="traced"):
+        make_fx(lambda x: call(x, *ins[1:]))(ins[0])
+    with pytest.raises(NotImplementedError, match="traced"):
+        torch.jit.trace(lambda x: call(x, *ins[1:]), (ins[0],))
+    leaf = ins[0].clone().requires_grad_()
+    out = call(leaf, *ins[1:])
+    out = out[0] if isinstance(out, tuple) else out
+    with pytest.raises(NotImplementedError, match="traced"):
+        make_fx(lambda dy: torch.autograd.grad(out, leaf, dy, retain_graph=True)[0])(torch.ones_like(out))
+    assert torch.isfinite(torch.autograd.grad(out, leaf, torch.ones_like(out))[0]).all()
+
+
+@pytest.mark.parametrize("name", MAKE)
+def test_a_mode_that_counts(name):
+    from torch.utils.flop_counter import FlopCounterMode
+
+    call, ins = MAKE[name]()
+    first = lambda out: out[0] if isinstance(out, tuple) else out             # noqa: E731
+    want = first(call(*ins))
+    with FlopCounterMode(display=False):
+        got = first(call(*ins))
+    assert torch.equal(got, want)
