@@ -96,3 +96,23 @@ def test_a_mode_that_counts(name):
     with FlopCounterMode(display=False):
         got = first(call(*ins))
     assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("name", MAKE)
+@pytest.mark.parametrize("way", ["extension"], indirect=True)
+def test_a_compiled_caller(name, way):
+    """A compiler that captures what it can runs the extension's call as it is, between its captured parts."""
+    call, ins = MAKE[name]()
+    first = lambda out: out[0] if isinstance(out, tuple) else out             # noqa: E731
+
+    def block(*a):
+        return first(call(*(t * 1 for t in a))) + 1
+
+    leaves = [t.clone().requires_grad_() for t in ins]
+    want = block(*leaves)
+    dy = torch.ones_like(want)
+    grads = torch.autograd.grad(want, leaves, dy)
+    torch._dynamo.reset()
+    got = torch.compile(block, backend="eager")(*leaves)
+    assert torch.equal(got, want)
+    assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(got, leaves, dy), grads))
