@@ -151,13 +151,20 @@ template <typename T> __host__ __device__ constexpr uint32_t idesc_of(bool a_mn,
 // ---------------------------------------------------------------- activation
 
 // act(a) and, where wanted, act'(a). Both are a times a logistic function: silu s(a), gelu's tanh form s(2 z) with
-// z = sqrt(2 / pi) (a + 0.044715 a^3). Beyond |a| = 16 the latter is 0 or 1 to 32 bits; z stops there so that a^3 stays finite.
+// z = sqrt(2 / pi) (a + 0.044715 a^3). Beyond |a| = 16 the latter is 0 or 1 to 32 bits; z stops there so that a^3 stays finite
+// (by a clamp that leaves a NaN one: a slope of 0 in its place would keep it out of the gate's gradient).
 // (A template argument: with a branch on it inside the epilogue's loops the backward one took 250 us instead of 209, 8192 x 2048 x 5632.)
 // The exponential and the reciprocal are the approximate instructions: 2^-21, against results of 11 bits at most.
+__device__ __forceinline__ float clamp_or_nan(float x, float most) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(x), "f"(-most));
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(r), "f"(most));
+  return r;
+}
 __device__ __forceinline__ float logistic(float x) { return __fdividef(1.f, 1.f + __expf(-x)); }
 template <bool Gelu, bool Slope> __device__ __forceinline__ float activate(float a, float& slope) {
   if constexpr (Gelu) {
-    const float c = 0.7978845608028654f, t = fminf(fmaxf(a, -16.f), 16.f), t2 = t * t;
+    const float c = 0.7978845608028654f, t = clamp_or_nan(a, 16.f), t2 = t * t;
     const float s = logistic(2.f * c * t * fmaf(0.044715f, t2, 1.f));
     if constexpr (Slope) slope = fmaf(2.f * c * t * s * (1.f - s), fmaf(3.f * 0.044715f, t2, 1.f), s);
     return a * s;
