@@ -449,6 +449,7 @@ std::optional<std::tuple<Tensor, std::optional<Tensor>, int64_t>> recurrence(con
   else if (want_final) final = at::empty(state_shape, opt.dtype(at::kFloat));
   a.state = ptr<float>(s); a.o = o.data_ptr(); a.final_state = final ? ptr<float>(*final) : nullptr;
   if (gdn2_recurrence_forward(&a, dtype_code(v.scalar_type()), stream_on(v)) != GDN2_OK) return std::nullopt;
+  if (in_place && !state->is_inference()) state->unsafeGetTensorImpl()->bump_version();     // autograd sees that it was written
   return std::make_tuple(o, final, recurrence_launches(a));
 }
 

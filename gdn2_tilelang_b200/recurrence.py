@@ -174,6 +174,8 @@ def gated_recurrence_decode(v, g, w, state):
     K = _cabi.kernels()
     rows = [None if t is None else t.flatten(2) for t in (v, g, w)]
     o, _, _ = K.recurrence(*rows, state.view(B, -1), None, in_place=True)
+    if not state.is_inference():
+        torch.autograd.graph.increment_version(state)  # autograd sees that it was written
     K.maybe_check_device_status(v.device)
     return o.view(v.shape)
 
