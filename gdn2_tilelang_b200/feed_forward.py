@@ -30,7 +30,7 @@ def _check(x, w_gate, w_up, w_down, activation):
     if hidden == 0 or inner == 0 or w_down.shape[0] == 0:
         raise ValueError("hidden, inner and output sizes must be positive")
     if x.dtype not in (torch.bfloat16, torch.float16):
-        raise TypeError(f"unsupported dtype {x.dtype}; use float16 or bfloat16")
+        raise TypeError(f"unsupported dtype {x.dtype}; use float16 or bfloat16 (float32 weights: under torch.autocast)")
     if any(w.dtype != x.dtype for w in (w_gate, w_up, w_down)):
         raise TypeError("x and the weights must share one dtype")
     _cabi._require_cuda(x, w_gate, w_up, w_down)
@@ -63,16 +63,24 @@ class _GatedFeedForward(torch.autograd.Function):
         return dx, (dwg if need[1] else None), (dwu if need[2] else None), dwd, None
 
 
+def _autocast(*tensors):
+    """What ``nn.Linear`` would do inside an autocast region: operands of up to 32 bits in the region's type."""
+    to = torch.get_autocast_dtype("cuda")
+    return tuple(t.to(to) if t.is_cuda and t.dtype in (torch.float32, torch.float16, torch.bfloat16) else t for t in tensors)
+
+
 def gated_feed_forward(x, w_gate, w_up, w_down, activation="silu"):
     """``(act(x w_gate^T) * (x w_up^T)) w_down^T``; differentiable in reverse mode, once.
 
     ``x``: ``[..., hidden]``; ``w_gate, w_up``: ``[inner, hidden]``; ``w_down``: ``[out, inner]`` (the layout of ``nn.Linear``), all float16
-    or all bfloat16. ``activation``: ``"silu"`` or ``"gelu_tanh"``. Returns ``[..., out]``. What one product
+    or all bfloat16; inside ``torch.autocast`` they are cast to its type first, so float32 weights train there. ``activation``: ``"silu"`` or ``"gelu_tanh"``. Returns ``[..., out]``. What one product
     reads of another is rounded to the inputs' type, sums are float32; a graph keeps 6 bytes an inner channel and token.
 
     Any sizes and row strides. Rows that do not start on 16 bytes (a size that is not a multiple of 8, an odd slice) are copied
     first, in one launch for all operands.
     """
+    if torch.is_autocast_enabled("cuda"):
+        x, w_gate, w_up, w_down = _autocast(x, w_gate, w_up, w_down)
     if x.is_cuda and activation in _cabi.ACTIVATIONS:
         K = _cabi.kernels()
         call = getattr(getattr(K, "host", None), "feed_forward", None)
@@ -101,7 +109,8 @@ def gated_feed_forward(x, w_gate, w_up, w_down, activation="silu"):
 
 class GatedFeedForward(nn.Module):
     """``gated_feed_forward`` with its weights: ``gate_proj``, ``up_proj`` (``hidden -> intermediate``) and ``down_proj``
-    (``intermediate -> hidden``), ``nn.Linear`` modules without biases that hold the parameters."""
+    (``intermediate -> hidden``), ``nn.Linear`` modules without biases that hold the parameters. They are made in the default type:
+    convert the module to float16 or bfloat16, or call it inside ``torch.autocast``."""
 
     def __init__(self, hidden_size: int, intermediate_size: int, activation: str = "silu"):
         super().__init__()
