@@ -196,15 +196,6 @@ template <typename T> __device__ __forceinline__ void put_row(char* chunk, int l
     *reinterpret_cast<uint4*>(chunk + lane * 128 + (((first / 8 + j) ^ (lane & 7)) * 16)) = r;
   }
 }
-template <typename T> __device__ __forceinline__ void get_row(const char* chunk, int lane, int first, float (&x)[32]) {
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const uint4 r = *reinterpret_cast<const uint4*>(chunk + lane * 128 + (((first / 8 + j) ^ (lane & 7)) * 16));
-    const T* e = reinterpret_cast<const T*>(&r);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) x[8 * j + i] = to_f32<T>(e[i]);
-  }
-}
 // The upper 24 bits of two or four numbers, rounded (ties away from zero; a number within 2^-17 of the largest becomes infinite).
 // A NaN keeps its upper 16 bits, whose quiet bit is set.
 __device__ __forceinline__ uint32_t round24(float x) {
@@ -215,8 +206,7 @@ __device__ __forceinline__ uint32_t upper16(uint32_t b0, uint32_t b1) { return _
 __device__ __forceinline__ uint32_t lower8(uint32_t b0, uint32_t b1, uint32_t b2, uint32_t b3) {
   return __byte_perm(__byte_perm(b0, b1, 0x0051), __byte_perm(b2, b3, 0x0051), 0x5410);
 }
-// 32 columns from `first` (0 or 32) of this lane's row of a plane's chunk, from rounded numbers and back. The lower plane's rows
-// are 64 bytes, swizzled in 64-byte rows as TMA does it.
+// 32 columns from `first` (0 or 32) of this lane's row of the upper plane's chunk, from rounded numbers
 __device__ __forceinline__ void put_upper(char* chunk, int lane, int first, const uint32_t (&b)[32]) {
 #pragma unroll
   for (int j = 0; j < 4; ++j)
@@ -224,9 +214,8 @@ __device__ __forceinline__ void put_upper(char* chunk, int lane, int first, cons
         make_uint4(upper16(b[8 * j], b[8 * j + 1]), upper16(b[8 * j + 2], b[8 * j + 3]), upper16(b[8 * j + 4], b[8 * j + 5]),
                    upper16(b[8 * j + 6], b[8 * j + 7]));
 }
-__device__ __forceinline__ uint32_t lower_at(int lane, int j) { return lane * 64 + ((j ^ ((lane >> 1) & 3)) * 16); }
-// The backward epilogue's pieces are 32 columns: rows of 64 bytes of 16-bit elements (swizzled as TMA does it with rows of 64) and
-// of 32 bytes of the lower planes (with rows of 32).
+// Rows of 64 bytes, swizzled as TMA does it: of the forward chunk's lower planes, and of the backward epilogue's pieces, which are 32
+// columns (their lower planes have rows of 32 bytes).
 __device__ __forceinline__ uint32_t row64_at(int lane, int j) { return lane * 64 + ((j ^ ((lane >> 1) & 3)) * 16); }
 template <typename T> __device__ __forceinline__ void put_row64(char* piece, int lane, const float (&x)[32]) {
 #pragma unroll
@@ -571,8 +560,8 @@ product_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Proble
           chunk_free(lane);
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            *reinterpret_cast<uint4*>(chunk + lower_at(lane, j)) = make_uint4(alow[4 * j], alow[4 * j + 1], alow[4 * j + 2], alow[4 * j + 3]);
-            *reinterpret_cast<uint4*>(chunk + kChunkBytes / 2 + lower_at(lane, j)) =
+            *reinterpret_cast<uint4*>(chunk + row64_at(lane, j)) = make_uint4(alow[4 * j], alow[4 * j + 1], alow[4 * j + 2], alow[4 * j + 3]);
+            *reinterpret_cast<uint4*>(chunk + kChunkBytes / 2 + row64_at(lane, j)) =
                 make_uint4(ulow[4 * j], ulow[4 * j + 1], ulow[4 * j + 2], ulow[4 * j + 3]);
           }
           store_chunk<T>(chunk, &maps.kept[2], nullptr, 0, row, col, p.M, p.N, lane);

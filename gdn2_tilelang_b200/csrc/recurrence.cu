@@ -472,7 +472,6 @@ template <typename T, int VEC> struct Piece {                    // 16 bytes of 
   static_assert(VEC * sizeof(T) == 16, "a piece is 16 bytes");
   uint4 raw;
   __device__ __forceinline__ void load(const T* p) { raw = ld_stream(p); }
-  __device__ __forceinline__ void zero() { raw = make_uint4(0, 0, 0, 0); }
   __device__ __forceinline__ void get(float (&x)[VEC]) const {
     const T* e = reinterpret_cast<const T*>(&raw);
 #pragma unroll
@@ -489,7 +488,6 @@ template <typename T, int VEC> struct Piece {                    // 16 bytes of 
 template <typename T> struct Piece<T, 1> {
   T raw;
   __device__ __forceinline__ void load(const T* p) { raw = *p; }
-  __device__ __forceinline__ void zero() { raw = from_f32<T>(0.f); }
   __device__ __forceinline__ void get(float (&x)[1]) const { x[0] = to_f32<T>(raw); }
   static __device__ __forceinline__ void store(T* p, const float (&x)[1]) { *p = from_f32<T>(x[0]); }
 };
