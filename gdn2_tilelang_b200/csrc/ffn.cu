@@ -278,15 +278,6 @@ struct Shared {
   int abort;
 };
 
-// After a wait that ran out, copies and products of the block's own may still be on the way: they take microseconds, the block
-// stays two milliseconds before it gives up its memory. Called by every thread after a block barrier.
-__device__ __forceinline__ void after_a_failure(volatile int* abort) {
-  if (*abort) {
-    const long long t0 = clock64();
-    while (clock64() - t0 < 4000000) {}
-  }
-}
-
 // Tiles go in bands of 16 rows of tiles, down the rows first, so that the pairs at work at one time share operands in L2.
 __device__ __forceinline__ void tile_at(const Problem& p, int i, int& m, int& n) {
   const int band = 16, per = band * p.tiles_n, b = i / per, rows = min(band, p.tiles_m - b * band);
@@ -627,7 +618,7 @@ product_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Proble
   if constexpr (K == kPlain)
     if (split > 1) join_parts<T>(maps, p, sh, ring, staging, tmem, pair, (int)rank, part, split, status);
   __syncthreads();
-  after_a_failure(&sh.abort);
+  tc::after_a_failure(&sh.abort);
   cluster_sync();                                     // neither block leaves while the other's products or copies need it
   if (wid == 2)
     asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
@@ -751,7 +742,7 @@ __global__ void __launch_bounds__(kSkinnyThreads, 2) skinny_kernel(const __grid_
     }
   }
   __syncthreads();
-  after_a_failure(&sh.abort);
+  tc::after_a_failure(&sh.abort);
   if (CL > 1) cluster_sync();
   // every block finishes its share of the tile's rows for all tokens: the blocks' sums in their order
   {

@@ -153,6 +153,8 @@ template <int W, bool Back> struct Shared {
 // By one warp: the run of this block's tile goes to every block of the cluster; returns what enters this tile and moves `carry`
 // past the tiles of the whole cluster. Round `it` writes slots that the others read in round it - 2: nobody sends round it before
 // its own round it - 1 is complete, which every block entered only after reading round it - 2.
+// After a wait that ran out the rounds go on, so that every barrier is met, but what they exchange is arbitrary and their waits end at
+// once; it stays in the cluster's shared memory, which no block gives up before it has arrived (after_a_failure).
 template <typename Sh>
 __device__ __forceinline__ float2 enter_tile(Sh& sh, float4* slots, int64_t it, int rank, int CL, int lane, const Run& run,
                                              float2& carry, uint32_t* status) {
@@ -273,7 +275,7 @@ __global__ void __launch_bounds__(W * 32, W == 8 ? 3 : 1) scan_forward_kernel(co
   const int64_t tiles = (p.len + kTile - 1) / kTile, rounds = (tiles + p.CL - 1) / p.CL;
   auto fetch = [&](int64_t it, int s) {               // by one thread
     const int64_t tile = it * p.CL + p.rank;
-    if (tile < tiles) St::fetch(maps, tc::smem_u32(smem) + s * St::bytes, &sh.full[s], p, tile * kTile);
+    if (tile < tiles && !*static_cast<volatile int*>(&sh.abort)) St::fetch(maps, tc::smem_u32(smem) + s * St::bytes, &sh.full[s], p, tile * kTile);
   };
   if constexpr (Fed)
     if (tid == 0)
@@ -341,6 +343,7 @@ __global__ void __launch_bounds__(W * 32, W == 8 ? 3 : 1) scan_forward_kernel(co
   if (a.last && p.rank == 0 && wid == W - 1) ch.store(a.last + (int64_t)p.seq * a.D, carry);
   __syncthreads();
   if (p.CL > 1) cluster_sync();                       // no block leaves while another may still send to it
+  tc::after_a_failure(&sh.abort);
 }
 
 // ---------------------------------------------------------------- backward
@@ -370,7 +373,7 @@ __global__ void __launch_bounds__(W * 32, W == 8 ? 2 : 1) scan_backward_kernel(c
   const int64_t tiles = (p.len + kTile - 1) / kTile, rounds = (tiles + p.CL - 1) / p.CL;
   auto fetch = [&](int64_t it, int s) {
     const int64_t tile = tiles - 1 - (it * p.CL + p.rank);
-    if (tile >= 0) St::fetch(maps, tc::smem_u32(smem) + s * St::bytes, &sh.full[s], p, tile * kTile);
+    if (tile >= 0 && !*static_cast<volatile int*>(&sh.abort)) St::fetch(maps, tc::smem_u32(smem) + s * St::bytes, &sh.full[s], p, tile * kTile);
   };
   if constexpr (Fed)
     if (tid == 0)
@@ -459,6 +462,7 @@ __global__ void __launch_bounds__(W * 32, W == 8 ? 2 : 1) scan_backward_kernel(c
   if (a.last && p.rank == 0 && wid == 0) ch.store(a.last + (int64_t)p.seq * a.D, carry);
   __syncthreads();
   if (p.CL > 1) cluster_sync();
+  tc::after_a_failure(&sh.abort);
 }
 
 // ---------------------------------------------------------------- a thread's VEC neighbouring channels of one token

@@ -83,6 +83,15 @@ __device__ __forceinline__ void mbar_drain(uint64_t* bar, uint32_t parity) {
   while (!mbar_try_wait(bar, parity) && clock64() - t0 <= kWaitCycles) {}
 }
 
+// After a wait that ran out, copies and products of the block's own may still be on the way: they take microseconds, the block
+// stays two milliseconds before it gives up its memory. Called by every thread after a block barrier.
+__device__ __forceinline__ void after_a_failure(volatile int* abort) {
+  if (*abort) {
+    const long long t0 = clock64();
+    while (clock64() - t0 < 4000000) {}
+  }
+}
+
 // ------------------------------------------------------------------ proxy / tcgen05 fences
 
 __device__ __forceinline__ void fence_async_smem() {   // generic-proxy smem writes -> async proxy readers
