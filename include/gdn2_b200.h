@@ -430,7 +430,7 @@ int gdn2_oproj_reduce(const gdn2_oproj_reduce_args* args, int dtype, void* strea
  * token of a sequence, for the backward call. final_state may be state: decoding in place, S tokens at a time.
  * gdn2_recurrence_backward: dv, dw (NULL without w), dg [B, S, D] and dstate (may be NULL) from dout and dfinal_state (NULL:
  * zeros); v, g, w, state strides and marks as in the forward call.
- * Any D >= 1, B >= 1, S >= 1, any alignment of elements; 16-byte aligned rows of a multiple of 16 bytes take the fast kernels.
+ * Any D up to 2^24, B and S up to 2^30, any alignment of elements; 16-byte aligned rows of a multiple of 16 bytes take the fast kernels.
  * No counterpart in the reference, whose only token mixer is the delta rule's (its decay convention is this one's).
  */
 typedef struct gdn2_recurrence_args {
