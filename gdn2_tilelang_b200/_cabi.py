@@ -677,7 +677,7 @@ class NativeKernels:
     def aligned_rows(self, *matrices):
         """``[rows, cols]`` matrices of 16-bit elements as the tensor-core kernels read them: rows that start on 16 bytes and whose
         elements lie side by side. Those that do not are copied, all in one launch."""
-        out, copies = list(matrices), []
+        out, copies, sources = list(matrices), [], []
         for i, t in enumerate(matrices):
             if t.shape[1] > 1 and t.stride(1) != 1:
                 t = out[i] = t.contiguous()
@@ -685,6 +685,7 @@ class NativeKernels:
             if t.data_ptr() % 16 or (not one and (t.stride(0) % 8 or t.stride(0) < t.shape[1])):
                 pitch = -(-t.shape[1] // 8) * 8
                 out[i] = torch.empty(t.shape[0], pitch, dtype=t.dtype, device=t.device)[:, :t.shape[1]]
+                sources.append(t)        # alive until the launch: a next operand's memory must not be one's source
                 copies.append(RowCopy(t.data_ptr(), out[i].data_ptr(), *t.shape, 0 if one else t.stride(0), pitch))
         if copies:
             with _on_device(out[0].device):

@@ -457,6 +457,7 @@ std::optional<std::tuple<Tensor, std::optional<Tensor>, int64_t>> recurrence(con
 // copied, all in one launch. Returns whether one was.
 bool align_rows(std::vector<Tensor>& ms) {
   std::vector<gdn2_row_copy> copies;
+  std::vector<Tensor> sources;                       // alive until the launch: a next operand's memory must not be one's source
   for (Tensor& t : ms) {
     if (t.size(1) > 1 && t.stride(1) != 1) t = t.contiguous();
     const bool one = t.size(0) == 1;
@@ -464,6 +465,7 @@ bool align_rows(std::vector<Tensor>& ms) {
       const int64_t pitch = (t.size(1) + 7) / 8 * 8;
       Tensor d = at::empty({t.size(0), pitch}, t.options().requires_grad(false)).narrow(1, 0, t.size(1));
       copies.push_back({t.data_ptr(), d.data_ptr(), t.size(0), t.size(1), one ? 0 : t.stride(0), pitch});
+      sources.push_back(t);
       t = d;
     }
   }
