@@ -610,6 +610,13 @@ class NativeKernels:
 
     # -- diagonal recurrence -----------------------------------------------------------------
     @staticmethod
+    def _check_saved(ok: bool, what: str):
+        """A program's hooks may bring saved tensors back in another layout, which the backward passes lay out again; with another
+        type, shape or device they are no longer what the kernels read."""
+        if not ok:
+            raise RuntimeError(f"{what}: a saved tensor came back from a hook with another type, shape or device")
+
+    @staticmethod
     def _recurrence_args(v, g, w, offsets):
         """The argument structure with inputs and sizes filled in, and what has to stay alive until the call."""
         a = RecurrenceArgs()
@@ -657,8 +664,15 @@ class NativeKernels:
     def recurrence_backward(self, v, g, w, marks, do, dfinal, offsets, want_dstate):
         """``gdn2_recurrence_backward``: ``(dv, dg, dw | None, dstate | None)``."""
         _require_cuda(v, g, w, marks, do, dfinal)
-        a, keep = self._recurrence_args(v, g, w, offsets)
         dev = v.device
+        self._check_saved(v.dim() == 3 and g.shape == v.shape == do.shape and g.dtype == torch.float32 and do.dtype == v.dtype and
+                          (w is None or (w.shape == v.shape and w.dtype == v.dtype)) and
+                          all(t is None or t.device == dev for t in (g, w, marks, do, dfinal)), "gated_recurrence")
+        a, keep = self._recurrence_args(v, g, w, offsets)
+        rows = self.lib.gdn2_recurrence_marks(a.B, a.S, a.cu_seqlens, a.sequences)
+        self._check_saved(marks.dtype == torch.float32 and tuple(marks.shape) == (rows, a.D) and
+                          (dfinal is None or tuple(dfinal.shape) == (a.sequences, a.D)), "gated_recurrence")
+        marks = marks.contiguous()
         do, a.do_batch_stride, a.do_token_stride = _rows_view(do)
         dfinal = None if dfinal is None else dfinal.contiguous()
         dv = torch.empty(v.shape, dtype=v.dtype, device=dev)
@@ -721,7 +735,16 @@ class NativeKernels:
 
     def ffn_backward(self, x, w_gate, w_up, w_down, kept, dy, activation: str, want_dx: bool, want_dgate_up: bool, want_dw_down: bool):
         """``gdn2_ffn_backward``: ``(dx, dw_gate, dw_up, dw_down)``, ``None`` where not wanted."""
+        _require_cuda(x, w_gate, w_up, w_down, kept, dy)
+        ins = (x, w_gate, w_up, w_down)
+        self._check_saved(all(t.dim() == 2 and t.dtype == dy.dtype and t.device == dy.device for t in ins) and kept.device == dy.device and
+                          w_gate.shape[1] == x.shape[1] and w_up.shape == w_gate.shape and w_down.shape[1] == w_gate.shape[0] and
+                          tuple(dy.shape) == (x.shape[0], w_down.shape[0]), "gated_feed_forward")
+        x, w_gate, w_up, w_down, dy = self.aligned_rows(*ins, dy)
         a = self._ffn_args(x, w_gate, w_up, w_down, activation)
+        self._check_saved(kept.dtype == torch.uint8 and tuple(kept.shape) == (self.lib.gdn2_ffn_kept_bytes(a.tokens, a.inner_stride),),
+                          "gated_feed_forward")
+        kept = kept.contiguous()
         new = lambda *shape: torch.empty(*shape, dtype=x.dtype, device=x.device)                 # noqa: E731
         h, da, du = (new(a.tokens, a.inner_stride) for _ in range(3))
         dx = new(a.tokens, a.hidden) if want_dx else None

@@ -341,6 +341,15 @@ variable_list once(variable_list grads, const char* what) {
     if (t.defined()) t = live[i++];
   return grads;
 }
+// A program's hooks may bring saved tensors back in another layout, which the backward passes lay out again; with another type, shape
+// or device they are no longer what the kernels read.
+bool saved_as(const Tensor& t, const Tensor& like, at::ScalarType type, at::IntArrayRef sizes) {
+  return t.defined() && t.layout() == at::kStrided && t.device() == like.device() && t.scalar_type() == type && t.sizes() == sizes &&
+         !t.is_conj() && !t.is_neg();
+}
+void check_saved(bool ok, const char* what) {
+  TORCH_CHECK(ok, what, ": a saved tensor came back from a hook with another type, shape or device");
+}
 void* stream_on(const Tensor& t) { return c10::cuda::getCurrentCUDAStream(t.get_device()).stream(); }
 template <typename T> T* ptr(const Tensor& t) { return t.defined() ? static_cast<T*>(t.data_ptr()) : nullptr; }
 
@@ -393,10 +402,19 @@ struct Recurrence : torch::autograd::Function<Recurrence> {
     variable_list out(5);
     {
       at::NoGradGuard no_grad;
-      const Tensor &v = saved[0], &g = saved[1], &w = saved[2], &marks = saved[3];
-      const c10::cuda::CUDAGuard device(v.device());
+      const auto rows = [](const Tensor& t) { return t.defined() && t.dim() == 3 && t.size(2) > 1 && t.stride(2) != 1 ? t.contiguous() : t; };
+      const Tensor v = rows(saved[0]), g = rows(saved[1]), w = rows(saved[2]), marks = saved[3].contiguous();
+      const Tensor& given = grads[0].defined() ? grads[0] : grads[1];
       const std::vector<int64_t> offsets = ctx->saved_data["offsets"].toIntVector();
+      check_saved(v.dim() == 3 && saved_as(v, given, v.scalar_type(), v.sizes()) && dtype_code(v.scalar_type()) >= 0 &&
+                      (!grads[0].defined() || saved_as(v, given, grads[0].scalar_type(), grads[0].sizes())) &&
+                      saved_as(g, given, at::kFloat, v.sizes()) && (!w.defined() || saved_as(w, given, v.scalar_type(), v.sizes())),
+                  "gated_recurrence");
+      const c10::cuda::CUDAGuard device(v.device());
       gdn2_recurrence_args a = recurrence_args(v, g, w, offsets);
+      check_saved(saved_as(marks, given, at::kFloat, {(int64_t)gdn2_recurrence_marks(a.B, a.S, a.cu_seqlens, a.sequences), a.D}) &&
+                      (!grads[1].defined() || (grads[1].dim() == 2 && grads[1].size(0) == a.sequences && grads[1].size(1) == a.D)),
+                  "gated_recurrence");
       const auto opt = v.options().requires_grad(false);
       Tensor dout = grads[0].defined() ? grads[0] : at::zeros(v.sizes(), opt);
       if (dout.size(2) > 1 && dout.stride(2) != 1) dout = dout.contiguous();
@@ -509,11 +527,18 @@ struct FeedForward : torch::autograd::Function<FeedForward> {
     refuse_transforms(grads, "gated_feed_forward");
     {
       at::NoGradGuard no_grad;
-      const std::vector<Tensor> in(saved.begin(), saved.begin() + 4);
-      const c10::cuda::CUDAGuard device(in[0].device());
+      std::vector<Tensor> in(saved.begin(), saved.begin() + 4);
       std::vector<Tensor> dy{grads[0]};
-      const bool copied = align_rows(dy);
+      bool ok = true;
+      for (const Tensor& t : in) ok = ok && t.dim() == 2 && saved_as(t, dy[0], dy[0].scalar_type(), t.sizes());
+      check_saved(ok && in[1].size(1) == in[0].size(1) && in[2].sizes() == in[1].sizes() && in[3].size(1) == in[1].size(0) &&
+                      dy[0].sizes() == at::IntArrayRef({in[0].size(0), in[3].size(0)}),
+                  "gated_feed_forward");
+      const c10::cuda::CUDAGuard device(in[0].device());
+      const int copied = (int)align_rows(dy) + (int)align_rows(in);
       gdn2_ffn_args a = ffn_args(in, ctx->saved_data["activation"].toInt());
+      const Tensor kept = saved[4].contiguous();
+      check_saved(saved_as(kept, dy[0], at::kByte, {(int64_t)gdn2_ffn_kept_bytes(a.tokens, a.inner_stride)}), "gated_feed_forward");
       const auto opt = in[0].options().requires_grad(false);
       const bool dx = ctx->needs_input_grad(0), dgate = ctx->needs_input_grad(1), dup = ctx->needs_input_grad(2), ddown = ctx->needs_input_grad(3);
       const Tensor h = at::empty({a.tokens, a.inner_stride}, opt), da = at::empty_like(h), du = at::empty_like(h);
@@ -523,7 +548,7 @@ struct FeedForward : torch::autograd::Function<FeedForward> {
         out[2] = at::empty({a.inner, a.hidden}, opt);
       }
       if (ddown) out[3] = at::empty({a.out, a.inner}, opt);
-      a.h = h.data_ptr(); a.kept = saved[4].data_ptr(); a.dy = dy[0].data_ptr(); a.dy_stride = pitch_of(dy[0]);
+      a.h = h.data_ptr(); a.kept = kept.data_ptr(); a.dy = dy[0].data_ptr(); a.dy_stride = pitch_of(dy[0]);
       a.da = da.data_ptr(); a.du = du.data_ptr(); a.dx = ptr<void>(out[0]); a.dx_stride = a.hidden;
       a.dw_gate = ptr<void>(out[1]); a.dw_up = ptr<void>(out[2]); a.dw_down = ptr<void>(out[3]);
       check(gdn2_ffn_backward(&a, dtype_code(in[0].scalar_type()), stream_on(in[0])), "gdn2_ffn_backward");

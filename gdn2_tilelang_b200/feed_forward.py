@@ -57,7 +57,6 @@ class _GatedFeedForward(torch.autograd.Function):
         _cabi.refuse_tracing("gated_feed_forward")
         _cabi.refuse_tangents("gated_feed_forward", dy)
         need = ctx.needs_input_grad
-        dy = K.aligned_rows(dy)[0]
         dx, dwg, dwu, dwd = K.ffn_backward(*ctx.saved_tensors, dy, ctx.activation, need[0], need[1] or need[2], need[3])
         K.maybe_check_device_status(dy.device)
         return dx, (dwg if need[1] else None), (dwu if need[2] else None), dwd, None
